@@ -437,6 +437,80 @@ vc_status vc_cuda_transpose_last2(const float* in, float* out, size_t batch, siz
  *    library's one stream are ordered and safe. */
 vc_status vc_cuda_reduce_sum_noalloc(const float* in, size_t count, float* out);
 
+/* ---- language-model operators: norm, 8-bit product, sampling ----------------
+ * No counterpart in the reference. Together they take a residual stream to the
+ * next token: rms_norm_q8 -> matmul_q8 (the head) -> sample; rms_norm and its
+ * backward are the norm's training step, next to the cross-entropy above.
+ *
+ * An 8-bit matrix ("q8") holds int8 values, row-major, `pitch` bytes between
+ * rows; pitch is at least the row's length and a multiple of 16, the base is
+ * 16-byte aligned (pool blocks are), and every row has a float scale: value
+ * j of row i stands for q[i * pitch + j] * scale[i]. The entry points that
+ * write q8 rows zero the bytes past the row's length; matmul_q8 ignores them.
+ * A stride argument counts elements between the starts of rows (the row's
+ * length for a contiguous tensor). */
+
+/* h = x + residual (residual may be NULL: h = x),
+ * rstd = 1 / sqrt(mean(h^2) + eps), y = (h * rstd) * weight, each row of
+ * [rows, cols] by itself. h and rstd may be NULL when not wanted (the backward
+ * needs both, or x in h's place without a residual); h may be x or residual
+ * itself where that is contiguous, for a residual stream updated in place.
+ * Squares are summed in float by fours and then in double. */
+vc_status vc_cuda_rms_norm(const float* x, size_t x_stride, const float* residual, size_t residual_stride,
+                           const float* weight, size_t rows, size_t cols, float eps, float* h, float* y,
+                           float* rstd);
+
+/* Gradients of (h, y) = rms_norm for the upstreams gy of y and gh of h (gh may
+ * be NULL: zero): with t = gy * weight,
+ * dh = rstd * (t - h * (rstd^2 * mean(t * h))) + gh -- the gradient of x and of
+ * residual alike -- and dw[j] = sum over rows of gy * (h * rstd). dh or dw may
+ * be NULL to skip. All tensors contiguous; dh may be gy or gh itself. */
+vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const float* rstd, const float* gy,
+                                    const float* gh, size_t rows, size_t cols, float* dh, float* dw);
+
+/* rms_norm with y in 8 bits: u = h * weight, M = the row's max |u|,
+ * q = round(u * (127 / M)) (ties to even), scale = (M / 127) * rstd. rstd is a
+ * factor of the whole row, so q does not depend on it. A row whose M is below
+ * 2^-100 becomes zeros with scale 0; a row with an infinity or NaN becomes
+ * zeros with scale NaN, so that it shows in whatever is computed from it.
+ * h may be NULL, or x or residual itself as in vc_cuda_rms_norm. */
+vc_status vc_cuda_rms_norm_q8(const float* x, size_t x_stride, const float* residual, size_t residual_stride,
+                              const float* weight, size_t rows, size_t cols, float eps, float* h, int8_t* q,
+                              size_t q_pitch, float* scale);
+
+/* Rows of x in 8 bits by the same rule without the norm: M = the row's max
+ * |x|, q = round(x * (127 / M)), scale = M / 127. For weights (a scale for
+ * each output channel) and for activations that no norm precedes. */
+vc_status vc_cuda_quantize_q8(const float* x, size_t x_stride, size_t rows, size_t cols, int8_t* q, size_t q_pitch,
+                              float* scale);
+
+/* out [m, n] = (a b^T) * (a_scale[i] * b_scale[j]) + bias[j] for q8 matrices
+ * a [m, k] (activations, a scale for each token) and b [n, k] (weights, a
+ * scale for each output channel); bias may be NULL. The sums are exact 32-bit
+ * integers: k <= 131071, larger fails with VC_ERR_OVERFLOW. k = 0 gives the
+ * bias alone. */
+vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scale, const int8_t* b, size_t b_pitch,
+                            const float* b_scale, const float* bias, size_t m, size_t n, size_t k, float* out);
+
+/* The next token of each row of logits [rows, vocab], drawn from
+ * softmax(logits / temperature) as the filters leave it, with the given
+ * standard-exponential random numbers noise [rows, vocab] (positive).
+ * temperature, top_k, top_p and min_p are device arrays with a value for each
+ * row, or NULL for "off" (temperature 1). With m the row's maximum and
+ * w = e^((l - m) / temperature), classes are ordered by logit, equal ones by
+ * index, and these stay in the race: the first top_k (<= 0: off); of these the
+ * ones whose predecessors hold less than top_p of the mass (>= 1 or NaN: off);
+ * of these the ones with w >= min_p (NaN: off); and always the first. The token
+ * is the class with the largest w / noise, the lowest index of equal ones:
+ * class i with probability w_i / (sum of w in the race). A temperature that is
+ * not above 0 takes the first class in order (greedy; logprob at temperature
+ * 1). NaN and -inf logits are masked: never drawn. logprob is the token's under
+ * softmax(logits / temperature) before the filters. A row with every class
+ * masked gives token -1 and logprob NaN. vocab <= 2^23. */
+vc_status vc_cuda_sample(const float* logits, size_t logits_stride, const float* noise, size_t noise_stride,
+                         const float* temperature, const int64_t* top_k, const float* top_p, const float* min_p,
+                         size_t rows, size_t vocab, int64_t* token, float* logprob);
+
 #ifdef __cplusplus
 }
 #endif

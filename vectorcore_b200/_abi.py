@@ -112,6 +112,14 @@ _SIGS = {
     "vc_cuda_bias_relu_sum_backward": (c_int, [_f, _f, _f, c_size_t, c_size_t, _f, _f, c_void_p]),
     "vc_cuda_matmul": (c_int, [_f, _f, _f, c_size_t, c_size_t, c_size_t, _szp, _szp, c_size_t, c_int, c_int]),
     "vc_cuda_transpose_last2": (c_int, [_f, _f, c_size_t, c_size_t, c_size_t]),
+    "vc_cuda_rms_norm": (c_int, [_f, c_size_t, _f, c_size_t, _f, c_size_t, c_size_t, c_float, _f, _f, _f]),
+    "vc_cuda_rms_norm_backward": (c_int, [_f, _f, _f, _f, _f, c_size_t, c_size_t, _f, _f]),
+    "vc_cuda_rms_norm_q8": (c_int, [_f, c_size_t, _f, c_size_t, _f, c_size_t, c_size_t, c_float, _f, c_void_p,
+                                    c_size_t, _f]),
+    "vc_cuda_quantize_q8": (c_int, [_f, c_size_t, c_size_t, c_size_t, c_void_p, c_size_t, _f]),
+    "vc_cuda_matmul_q8": (c_int, [c_void_p, c_size_t, _f, c_void_p, c_size_t, _f, _f, c_size_t, c_size_t, c_size_t,
+                                  _f]),
+    "vc_cuda_sample": (c_int, [_f, c_size_t, _f, c_size_t, _f, c_void_p, _f, _f, c_size_t, c_size_t, c_void_p, _f]),
     "vc_cuda_reduce_sum_noalloc": (c_int, [_f, c_size_t, _f]),
     "vc_cuda_selftest_wait_timeout": (c_int, [c_int64]),
     "vc_cuda_reduce_axis_partial": (c_int, [c_int, _f, c_size_t, c_size_t, c_size_t, c_int64, c_int, c_void_p,

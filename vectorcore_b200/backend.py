@@ -23,6 +23,7 @@ from ._abi import EXP, LOG, NEG, RELU, RELU_GRAD, SIGMOID  # noqa: F401
 from ._abi import REDUCE_ARGMAX, REDUCE_MAX, REDUCE_MEAN, REDUCE_SUM  # noqa: F401
 
 _F32 = 4
+_FLOAT32, _INT64, _INT8 = np.dtype(np.float32), np.dtype(np.int64), np.dtype(np.int8)
 
 
 class CudaStorage:
@@ -30,7 +31,7 @@ class CudaStorage:
     modification counter shared by every view (storage.hpp:22-23).
 
     ``dtype`` is float32 except for the int64 index / target buffers the
-    fused kernels use."""
+    fused kernels use and the int8 values of 8-bit matrices."""
 
     __slots__ = ("ptr", "size", "dtype", "version", "__weakref__")
 
@@ -39,6 +40,16 @@ class CudaStorage:
         self.size = int(elements)
         self.version = 0
         self.ptr = _abi.alloc(max(self.size, 1) * self.dtype.itemsize)
+
+    @classmethod
+    def borrow(cls, ptr: int, elements: int, dtype=_FLOAT32) -> "CudaStorage":
+        """A storage over device memory that somebody else owns (another
+        library's tensor, part of a larger buffer): nothing is allocated, and
+        nothing is freed when it goes. The owner keeps the memory until the
+        work enqueued on it is done."""
+        s = _Borrowed.__new__(_Borrowed)
+        s.ptr, s.size, s.dtype, s.version = ptr, elements, dtype, 0
+        return s
 
     @property
     def nbytes(self) -> int:
@@ -59,9 +70,41 @@ class CudaStorage:
         return "cuda"
 
 
+class _Borrowed(CudaStorage):
+    __slots__ = ()
+
+    def __del__(self):
+        pass
+
+
 def _p(x):
     """Raw device address of a storage (or None)."""
     return None if x is None else ctypes.c_void_p(x.ptr)
+
+
+def _at(x, elements, dtype, what):
+    """Raw device address of a storage that has to hold `elements` of `dtype`
+    (None stays None)."""
+    if x is None:
+        return None
+    if x.dtype != dtype:
+        raise ValueError(f"{what} is {x.dtype}, not {dtype}")
+    if x.size < elements:
+        raise IndexError(f"{what} has {x.size} elements, {elements} are needed")
+    return x.ptr
+
+
+def _span(rows, cols, stride):
+    """Elements from the first of `rows` rows to the end of the last."""
+    if rows < 0 or cols < 0 or stride < 0:
+        raise ValueError("sizes and strides are not negative")
+    return (rows - 1) * stride + cols if rows else 0
+
+
+def q8_pitch(cols: int) -> int:
+    """Bytes between the rows of an 8-bit matrix with `cols` columns: rows
+    start on 16-byte boundaries."""
+    return (cols + 15) // 16 * 16
 
 
 class PinnedBuffer:
@@ -150,6 +193,13 @@ class CudaBackend:
     def synchronize(self) -> None:
         _abi.synchronize()
 
+    def use_stream(self, handle: int | None) -> None:
+        """Enqueue on the stream with this raw handle from now on (another
+        library's, e.g. torch.cuda.Stream.cuda_stream; 0 is the default
+        stream). None goes back to the device's own stream."""
+        # NULL restores the own stream in the C ABI; 1 is cudaStreamLegacy
+        _abi.call("vc_cuda_set_stream", ctypes.c_void_p(None if handle is None else handle or 1))
+
     def capture(self, fn):
         """Run fn() under stream capture; returns (CudaGraph, fn's result).
         The captured work is NOT executed by the capture itself: launch the
@@ -173,9 +223,11 @@ class CudaBackend:
     def allocate(self, elements: int, dtype=np.float32) -> CudaStorage:
         return CudaStorage(elements, dtype)
 
-    def upload(self, values: np.ndarray) -> CudaStorage:
-        values = np.ascontiguousarray(values)
-        if values.dtype not in (np.float32, np.int64):
+    def upload(self, values: np.ndarray, dtype=None) -> CudaStorage:
+        """Copy to the device as float32, or int64 where the values are that;
+        `dtype` keeps another type (np.int8: the values of an 8-bit matrix)."""
+        values = np.ascontiguousarray(values, dtype)
+        if dtype is None and values.dtype not in (np.float32, np.int64):
             values = values.astype(np.float32)
         s = CudaStorage(values.size, values.dtype)
         _abi.call("vc_cuda_upload", ctypes.c_void_p(s.ptr), values.ctypes.data_as(ctypes.c_void_p),
@@ -379,3 +431,93 @@ class CudaBackend:
         _abi.call("vc_cuda_bias_relu_sum_backward", _p(x), _p(b), _p(upstream), ctypes.c_size_t(rows),
                   ctypes.c_size_t(cols), _p(dx), _p(db), None)
         return dx, db
+
+    # ---- language-model operators: norm, 8-bit product, sampling --------------
+    # `out` takes the storages to write (a loop that must not allocate);
+    # without it they come from the pool like every other result.
+    def rms_norm(self, x, weight, rows, cols, eps=1e-6, residual=None, x_stride=None, residual_stride=None,
+                 out=None):
+        """(y, h, rstd) of h = x + residual, rstd = 1 / sqrt(mean(h^2) + eps),
+        y = h * rstd * weight, row by row. Without a residual h is x, and the
+        h returned is None unless `out` has a storage for it."""
+        xs = cols if x_stride is None else x_stride
+        rs = cols if residual_stride is None else residual_stride
+        n = _span(rows, cols, cols)
+        if out is None:
+            out = (CudaStorage(n), CudaStorage(n) if residual is not None else None, CudaStorage(rows))
+        y, h, rstd = out
+        _abi.call("vc_cuda_rms_norm", _at(x, _span(rows, cols, xs), _FLOAT32, "x"), xs,
+                  _at(residual, _span(rows, cols, rs), _FLOAT32, "residual"), rs, _at(weight, cols, _FLOAT32, "weight"),
+                  rows, cols, eps, _at(h, n, _FLOAT32, "h"), _at(y, n, _FLOAT32, "y"),
+                  _at(rstd, rows, _FLOAT32, "rstd"))
+        return out
+
+    def rms_norm_backward(self, h, weight, rstd, gy, rows, cols, gh=None, need_w=True, out=None):
+        """(dh, dw) for the upstream gradients gy of y and gh of h (None:
+        zero); dh is the gradient of x and of the residual alike."""
+        n = _span(rows, cols, cols)
+        if out is None:
+            out = (CudaStorage(n), CudaStorage(cols) if need_w else None)
+        dh, dw = out
+        _abi.call("vc_cuda_rms_norm_backward", _at(h, n, _FLOAT32, "h"), _at(weight, cols, _FLOAT32, "weight"),
+                  _at(rstd, rows, _FLOAT32, "rstd"), _at(gy, n, _FLOAT32, "gy"), _at(gh, n, _FLOAT32, "gh"), rows, cols,
+                  _at(dh, n, _FLOAT32, "dh"), _at(dw, cols, _FLOAT32, "dw"))
+        return out
+
+    def rms_norm_q8(self, x, weight, rows, cols, eps=1e-6, residual=None, x_stride=None, residual_stride=None,
+                    out=None):
+        """(q, scale, h): rms_norm with y as an 8-bit matrix, its rows
+        q8_pitch(cols) bytes apart."""
+        xs = cols if x_stride is None else x_stride
+        rs = cols if residual_stride is None else residual_stride
+        n, pitch = _span(rows, cols, cols), q8_pitch(cols)
+        if out is None:
+            out = (CudaStorage(rows * pitch, _INT8), CudaStorage(rows), CudaStorage(n) if residual is not None else None)
+        q, scale, h = out
+        _abi.call("vc_cuda_rms_norm_q8", _at(x, _span(rows, cols, xs), _FLOAT32, "x"), xs,
+                  _at(residual, _span(rows, cols, rs), _FLOAT32, "residual"), rs, _at(weight, cols, _FLOAT32, "weight"),
+                  rows, cols, eps, _at(h, n, _FLOAT32, "h"), _at(q, rows * pitch, _INT8, "q"), pitch,
+                  _at(scale, rows, _FLOAT32, "scale"))
+        return out
+
+    def quantize_q8(self, x, rows, cols, x_stride=None, out=None):
+        """(q, scale): the rows of x as an 8-bit matrix, rows q8_pitch(cols)
+        bytes apart."""
+        xs, pitch = cols if x_stride is None else x_stride, q8_pitch(cols)
+        need = _span(rows, cols, xs)
+        if out is None:
+            out = (CudaStorage(rows * pitch, _INT8), CudaStorage(rows))
+        q, scale = out
+        _abi.call("vc_cuda_quantize_q8", _at(x, need, _FLOAT32, "x"), xs, rows, cols, _at(q, rows * pitch, _INT8, "q"),
+                  pitch, _at(scale, rows, _FLOAT32, "scale"))
+        return out
+
+    def matmul_q8(self, a, a_scale, b, b_scale, m, n, k, bias=None, a_pitch=None, b_pitch=None, out=None):
+        """out [m, n] = (a b^T) * a_scale * b_scale (+ bias) for 8-bit matrices
+        a [m, k] and b [n, k], rows q8_pitch(k) bytes apart by default."""
+        ap = q8_pitch(k) if a_pitch is None else a_pitch
+        bp = q8_pitch(k) if b_pitch is None else b_pitch
+        na, nb = _span(m, k, ap), _span(n, k, bp)
+        if out is None:
+            out = CudaStorage(m * n)
+        _abi.call("vc_cuda_matmul_q8", _at(a, na, _INT8, "a"), ap, _at(a_scale, m, _FLOAT32, "a_scale"),
+                  _at(b, nb, _INT8, "b"), bp, _at(b_scale, n, _FLOAT32, "b_scale"), _at(bias, n, _FLOAT32, "bias"), m, n, k,
+                  _at(out, m * n, _FLOAT32, "out"))
+        return out
+
+    def sample(self, logits, noise, rows, vocab, temperature=None, top_k=None, top_p=None, min_p=None,
+               row_stride=None, noise_stride=None, out=None):
+        """(token int64, logprob) of each row of logits [rows, vocab]; noise
+        holds standard-exponential random numbers, the settings a value for
+        each row (top_k int64) or None for off."""
+        ls = vocab if row_stride is None else row_stride
+        ns = vocab if noise_stride is None else noise_stride
+        nl, nn = _span(rows, vocab, ls), _span(rows, vocab, ns)
+        if out is None:
+            out = (CudaStorage(rows, _INT64), CudaStorage(rows))
+        token, logprob = out
+        _abi.call("vc_cuda_sample", _at(logits, nl, _FLOAT32, "logits"), ls, _at(noise, nn, _FLOAT32, "noise"), ns,
+                  _at(temperature, rows, _FLOAT32, "temperature"), _at(top_k, rows, _INT64, "top_k"),
+                  _at(top_p, rows, _FLOAT32, "top_p"), _at(min_p, rows, _FLOAT32, "min_p"), rows, vocab,
+                  _at(token, rows, _INT64, "token"), _at(logprob, rows, _FLOAT32, "logprob"))
+        return out

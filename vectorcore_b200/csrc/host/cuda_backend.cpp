@@ -270,6 +270,74 @@ std::shared_ptr<Storage> CudaBackend::cross_entropy_backward(const Storage& logi
     return out;
 }
 
+namespace {
+
+// 8-bit rows start on 16-byte boundaries.
+std::size_t q8_pitch(std::size_t cols) { return (cols + 15) / 16 * 16; }
+
+const float* optional(const Storage* s) { return s ? ptr(*s) : nullptr; }
+
+std::int8_t* q8_ptr(const Storage& s) { return static_cast<std::int8_t*>(as_cuda(s).raw()); }
+
+}  // namespace
+
+CudaBackend::NormResult CudaBackend::rms_norm(const Storage& x, const Storage* residual, const Storage& weight,
+                                              std::size_t rows, std::size_t cols, float eps) {
+    NormResult r{make(rows * cols, device_), residual ? make(rows * cols, device_) : nullptr, make(rows, device_)};
+    check(vc_cuda_rms_norm(ptr(x), cols, optional(residual), cols, ptr(weight), rows, cols, eps,
+                           r.h ? ptr(*r.h) : nullptr, ptr(*r.y), ptr(*r.rstd)),
+          "rms_norm failed");
+    return r;
+}
+
+CudaBackend::NormGradients CudaBackend::rms_norm_backward(const Storage& h, const Storage& weight, const Storage& rstd,
+                                                          const Storage& gy, const Storage* gh, std::size_t rows,
+                                                          std::size_t cols) {
+    NormGradients r{make(rows * cols, device_), make(cols, device_)};
+    check(vc_cuda_rms_norm_backward(ptr(h), ptr(weight), ptr(rstd), ptr(gy), optional(gh), rows, cols, ptr(*r.dh),
+                                    ptr(*r.dw)),
+          "rms_norm_backward failed");
+    return r;
+}
+
+CudaBackend::NormQ8Result CudaBackend::rms_norm_q8(const Storage& x, const Storage* residual, const Storage& weight,
+                                                   std::size_t rows, std::size_t cols, float eps) {
+    const std::size_t pitch = q8_pitch(cols);
+    NormQ8Result r{{make(rows * pitch, device_, 1), make(rows, device_), rows, cols, pitch},
+                   residual ? make(rows * cols, device_) : nullptr};
+    check(vc_cuda_rms_norm_q8(ptr(x), cols, optional(residual), cols, ptr(weight), rows, cols, eps,
+                              r.h ? ptr(*r.h) : nullptr, q8_ptr(*r.q.values), pitch, ptr(*r.q.scale)),
+          "rms_norm_q8 failed");
+    return r;
+}
+
+CudaBackend::Q8Matrix CudaBackend::quantize_q8(const Storage& x, std::size_t rows, std::size_t cols) {
+    const std::size_t pitch = q8_pitch(cols);
+    Q8Matrix r{make(rows * pitch, device_, 1), make(rows, device_), rows, cols, pitch};
+    check(vc_cuda_quantize_q8(ptr(x), cols, rows, cols, q8_ptr(*r.values), pitch, ptr(*r.scale)), "quantize_q8 failed");
+    return r;
+}
+
+std::shared_ptr<Storage> CudaBackend::matmul_q8(const Q8Matrix& a, const Q8Matrix& b, const Storage* bias) {
+    if (a.cols != b.cols) throw std::invalid_argument("matmul_q8: rows of different lengths");
+    auto out = make(a.rows * b.rows, device_);
+    check(vc_cuda_matmul_q8(q8_ptr(*a.values), a.pitch, ptr(*a.scale), q8_ptr(*b.values), b.pitch, ptr(*b.scale),
+                            optional(bias), a.rows, b.rows, a.cols, out->device_data()),
+          "matmul_q8 failed");
+    return out;
+}
+
+CudaBackend::SampleResult CudaBackend::sample(const Storage& logits, const Storage& noise,
+                                              const SampleSettings& settings, std::size_t rows, std::size_t vocab) {
+    SampleResult r{make(rows, device_, sizeof(std::int64_t)), make(rows, device_)};
+    check(vc_cuda_sample(ptr(logits), vocab, ptr(noise), vocab, optional(settings.temperature),
+                         settings.top_k ? static_cast<const std::int64_t*>(as_cuda(*settings.top_k).raw()) : nullptr,
+                         optional(settings.top_p), optional(settings.min_p), rows, vocab,
+                         static_cast<std::int64_t*>(as_cuda(*r.token).raw()), ptr(*r.logprob)),
+          "sample failed");
+    return r;
+}
+
 bool cuda_available() { return CudaBackend::instance().available(); }
 
 std::string cuda_device_name() { return CudaBackend::instance().device_name(); }

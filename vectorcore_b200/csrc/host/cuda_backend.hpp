@@ -133,6 +133,45 @@ public:
                                                                   const Storage& upstream, std::size_t batch,
                                                                   std::size_t classes);
 
+    // ---- language-model operators (no counterpart in the reference) ---------
+    // A matrix of int8 values, `pitch` bytes between rows, and a float scale
+    // for each row (vc_cuda.h, "q8").
+    struct Q8Matrix {
+        std::shared_ptr<Storage> values, scale;
+        std::size_t rows, cols, pitch;
+    };
+    struct NormResult {
+        std::shared_ptr<Storage> y, h, rstd;  // h: null without a residual (it is x)
+    };
+    struct NormGradients {
+        std::shared_ptr<Storage> dh, dw;
+    };
+    struct NormQ8Result {
+        Q8Matrix q;
+        std::shared_ptr<Storage> h;  // null without a residual
+    };
+    struct SampleSettings {  // a value for each row, or null for off
+        const Storage* temperature{nullptr};
+        const Storage* top_k{nullptr};  // int64
+        const Storage* top_p{nullptr};
+        const Storage* min_p{nullptr};
+    };
+    struct SampleResult {
+        std::shared_ptr<Storage> token, logprob;  // token: int64
+    };
+    [[nodiscard]] NormResult rms_norm(const Storage& x, const Storage* residual, const Storage& weight,
+                                      std::size_t rows, std::size_t cols, float eps);
+    [[nodiscard]] NormGradients rms_norm_backward(const Storage& h, const Storage& weight, const Storage& rstd,
+                                                  const Storage& gy, const Storage* gh, std::size_t rows,
+                                                  std::size_t cols);
+    [[nodiscard]] NormQ8Result rms_norm_q8(const Storage& x, const Storage* residual, const Storage& weight,
+                                           std::size_t rows, std::size_t cols, float eps);
+    [[nodiscard]] Q8Matrix quantize_q8(const Storage& x, std::size_t rows, std::size_t cols);
+    // out [a.rows, b.rows] = a b^T with both scales (+ bias)
+    [[nodiscard]] std::shared_ptr<Storage> matmul_q8(const Q8Matrix& a, const Q8Matrix& b, const Storage* bias);
+    [[nodiscard]] SampleResult sample(const Storage& logits, const Storage& noise, const SampleSettings& settings,
+                                      std::size_t rows, std::size_t vocab);
+
 private:
     Device device_;
 };
