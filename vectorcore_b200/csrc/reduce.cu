@@ -1508,25 +1508,6 @@ static void launch_tma_nvt(unsigned nvt, const CUtensorMap& map, const float* a,
     }
 }
 
-// cuTensorMapEncodeTiled from the driver, looked up once through the runtime
-// (the library does not link libcuda).
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled() {
-    static EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            return static_cast<EncodeTiledFn>(nullptr);
-        }
-        return reinterpret_cast<EncodeTiledFn>(p);
-    }();
-    return fn;
-}
-
 // Launch bcast_backward_tma for a classified shape (FusedDesc filled by the
 // caller) when it qualifies; false, having launched nothing, otherwise.
 static bool try_tma_bcast_backward(int op, const float* a, const float* b, const float* g, const FusedDesc& fd,

@@ -3,6 +3,7 @@
 
 #include "vc_cuda.h"
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -70,6 +71,13 @@ constexpr std::size_t kCounterSlots = 1u << 16;
 constexpr unsigned kErrWaitTimeout = 1u << 0;   // a bounded wait gave up
 constexpr unsigned kErrBadTarget = 1u << 1;     // class target out of range
 constexpr unsigned kErrBadIndex = 1u << 2;      // scatter index out of range
+
+// cuTensorMapEncodeTiled from the driver, looked up once through the runtime
+// (the library does not link libcuda); null when the driver has none.
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled();
 
 // Stream-ordered scratch from the pool; returned to the pool on scope exit
 // (after the kernels that use it were enqueued, which stream order makes safe).
