@@ -74,29 +74,62 @@ __device__ __forceinline__ RowStats reduce_row(double sq, float amax, double* ss
     return RowStats{sq, amax};
 }
 
-template <int VEC>
-struct Group {
-    float v[VEC];
-};
-
-template <int VEC>
-__device__ __forceinline__ Group<VEC> load_group(const float* p, unsigned long long g) {
-    Group<VEC> o;
-    if constexpr (VEC == 4) {
-        const float4 f = reinterpret_cast<const float4*>(p)[g];
-        o.v[0] = f.x, o.v[1] = f.y, o.v[2] = f.z, o.v[3] = f.w;
-    } else {
-        o.v[0] = p[g];
+// A row in groups of four floats on the 16-byte grid of its address. Rows whose
+// length is no multiple of four start anywhere on it: with `skew` floats between
+// the grid and the row's start, group g holds the elements 4g - skew ..
+// 4g - skew + 3, and the first and last group may hold fewer.
+struct Span {
+    unsigned skew, cols;
+    __device__ __forceinline__ unsigned groups() const { return (skew + cols + 3) >> 2; }
+    __device__ __forceinline__ bool whole(unsigned g) const { return 4 * g >= skew && 4 * g + 4 <= skew + cols; }
+    __device__ __forceinline__ bool has(unsigned g, unsigned e) const {
+        return 4 * g + e >= skew && 4 * g + e < skew + cols;
     }
-    return o;
-}
+};
+struct Group {
+    float v[4];
+};
+__device__ __forceinline__ Group group_of(float4 f) { return Group{{f.x, f.y, f.z, f.w}}; }
 
-template <int VEC>
-__device__ __forceinline__ void store_group(float* p, unsigned long long g, const Group<VEC>& o) {
-    if constexpr (VEC == 4)
-        reinterpret_cast<float4*>(p)[g] = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
-    else
-        p[g] = o.v[0];
+// p: the row's start. SKEWED false: every row starts on the grid and ends on it.
+template <bool SKEWED>
+__device__ __forceinline__ Group load_group(const float* p, unsigned g, const Span& r) {
+    if constexpr (!SKEWED) {
+        return group_of(reinterpret_cast<const float4*>(p)[g]);
+    } else {
+        if (r.whole(g)) return group_of(*reinterpret_cast<const float4*>(p - r.skew + 4ull * g));
+        Group o;
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) o.v[e] = r.has(g, e) ? p[4 * g + e - r.skew] : 0.0f;
+        return o;
+    }
+}
+// The norm's weight, which no output overlaps: read-only loads can be issued
+// ahead of the stores (without that the forward ran at 45% of its speed). It
+// starts on the grid, so a skewed group is four loads.
+template <bool SKEWED>
+__device__ __forceinline__ Group load_weight(const float* w, unsigned g, const Span& r) {
+    if constexpr (!SKEWED) {
+        return group_of(__ldg(reinterpret_cast<const float4*>(w) + g));
+    } else {
+        Group o;
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e) o.v[e] = r.has(g, e) ? __ldg(w + (4 * g + e - r.skew)) : 0.0f;
+        return o;
+    }
+}
+template <bool SKEWED>
+__device__ __forceinline__ void store_group(float* p, unsigned g, const Group& o, const Span& r) {
+    const float4 f = make_float4(o.v[0], o.v[1], o.v[2], o.v[3]);
+    if constexpr (!SKEWED) {
+        reinterpret_cast<float4*>(p)[g] = f;
+    } else if (r.whole(g)) {
+        *reinterpret_cast<float4*>(p - r.skew + 4ull * g) = f;
+    } else {
+#pragma unroll
+        for (unsigned e = 0; e < 4; ++e)
+            if (r.has(g, e)) p[4 * g + e - r.skew] = o.v[e];
+    }
 }
 
 // max |u| as fmaxf, but a NaN stays: NaN compares false, so it is kept by the
@@ -124,9 +157,13 @@ __device__ __forceinline__ Q8Row q8_row(float amax, float rstd) {
 // u * inv rounds to at most 127: M * (127 / M) is below 127.00002.
 __device__ __forceinline__ int q8_value(float u, float inv) { return inv == 0.0f ? 0 : __float2int_rn(u * inv); }
 
+__device__ __forceinline__ unsigned skew_of(const float* p) {
+    return static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(p) >> 2) & 3;
+}
+
 // One row a CTA (or a row a warp, blockDim.y of them, for short rows): the row
-// is read once and stays in registers, NV groups of VEC floats a thread.
-template <int MODE, int VEC, int NV>
+// is read once and stays in registers, NV groups a thread.
+template <int MODE, bool SKEWED, int NV>
 __global__ void __launch_bounds__(1024)
 norm_kernel(const NormArgs a) {
     __shared__ double ssq[32];
@@ -134,26 +171,24 @@ norm_kernel(const NormArgs a) {
     const unsigned long long row = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;  // whole warps: blockDim.y > 1 only with one warp a row
     const unsigned T = blockDim.x, t = threadIdx.x;
-    const unsigned G = a.cols / VEC;  // VEC divides cols
     const float* x = a.x + row * a.xs;
     const float* r = a.r ? a.r + row * a.rs : nullptr;
-    Group<VEC> h[NV];
+    const Span span{SKEWED ? skew_of(x) : 0, a.cols};
+    const unsigned G = span.groups();
+    Group h[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const unsigned g = t + i * T;
-        if (g < G) h[i] = load_group<VEC>(x, g);
-        else
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) h[i].v[e] = 0.0f;
+        h[i] = g < G ? load_group<SKEWED>(x, g, span) : Group{};
     }
     if (r) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const unsigned g = t + i * T;
             if (g < G) {
-                const Group<VEC> o = load_group<VEC>(r, g);
+                const Group o = load_group<SKEWED>(r, g, span);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) h[i].v[e] += o.v[e];
+                for (int e = 0; e < 4; ++e) h[i].v[e] += o.v[e];
             }
         }
     }
@@ -163,19 +198,19 @@ norm_kernel(const NormArgs a) {
     for (int i = 0; i < NV; ++i) {
         const unsigned g = t + i * T;
         if (g < G) {
-            if (a.h) store_group<VEC>(a.h + row * a.cols, g, h[i]);
+            if (a.h) store_group<SKEWED>(a.h + row * a.cols, g, h[i], span);
             float part = 0.0f;
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) part = fmaf(h[i].v[e], h[i].v[e], part);
+            for (int e = 0; e < 4; ++e) part = fmaf(h[i].v[e], h[i].v[e], part);
             if (MODE != QUANT_Q8) sq += part;
             if (MODE == NORM_Q8) {
-                const Group<VEC> w = load_group<VEC>(a.w, g);
+                const Group w = load_weight<SKEWED>(a.w, g, span);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) h[i].v[e] *= w.v[e];
+                for (int e = 0; e < 4; ++e) h[i].v[e] *= w.v[e];
             }
             if (MODE != NORM_F32)
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) amax = amax_nan(amax, fabsf(h[i].v[e]));
+                for (int e = 0; e < 4; ++e) amax = amax_nan(amax, fabsf(h[i].v[e]));
         }
     }
     // a NaN maximum survives the fmaxf tree as infinity (both poison the row)
@@ -189,10 +224,10 @@ norm_kernel(const NormArgs a) {
         for (int i = 0; i < NV; ++i) {
             const unsigned g = t + i * T;
             if (g < G) {
-                const Group<VEC> w = load_group<VEC>(a.w, g);
+                const Group w = load_weight<SKEWED>(a.w, g, span);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) h[i].v[e] = h[i].v[e] * rstd * w.v[e];
-                store_group<VEC>(y, g, h[i]);
+                for (int e = 0; e < 4; ++e) h[i].v[e] = h[i].v[e] * rstd * w.v[e];
+                store_group<SKEWED>(y, g, h[i], span);
             }
         }
     } else {
@@ -202,13 +237,30 @@ norm_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const unsigned g = t + i * T;
-            if (g < G) {
-                if constexpr (VEC == 4)
-                    reinterpret_cast<char4*>(q)[g] =
-                        make_char4(q8_value(h[i].v[0], o.inv), q8_value(h[i].v[1], o.inv), q8_value(h[i].v[2], o.inv),
-                                   q8_value(h[i].v[3], o.inv));
-                else
-                    q[g] = static_cast<signed char>(q8_value(h[i].v[0], o.inv));
+            int v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = q8_value(h[i].v[e], o.inv);
+            if (!SKEWED) {
+                if (g < G) reinterpret_cast<char4*>(q)[g] = make_char4(v[0], v[1], v[2], v[3]);
+            } else {
+                // The row of q starts on the grid. Words of four values take
+                // the end of this lane's group and the beginning of the next
+                // lane's; a warp's two ends go out by bytes.
+                const unsigned lane = t & 31;
+                const unsigned mine = (v[0] & 255) | (v[1] & 255) << 8 | (v[2] & 255) << 16 |
+                                      static_cast<unsigned>(v[3]) << 24;
+                const unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
+                const unsigned at = 4 * g;  // the word's first element
+                if (lane < 31 && g < G && at + 4 <= a.cols)
+                    *reinterpret_cast<unsigned*>(q + at) = __funnelshift_r(mine, next, 8 * span.skew);
+#pragma unroll
+                for (unsigned e = 0; e < 4; ++e) {
+                    // by bytes: what the words above leave out
+                    const unsigned j = at + e - span.skew;
+                    const bool ahead = e < span.skew;  // in the word of the group before
+                    const bool out = ahead ? lane == 0 || (j & ~3u) + 4 > a.cols : lane == 31 || at + 4 > a.cols;
+                    if (g < G && span.has(g, e) && out) q[j] = static_cast<signed char>(v[e]);
+                }
             }
         }
         for (unsigned long long j = a.cols + t; j < a.pitch; j += T) q[j] = 0;
@@ -254,40 +306,64 @@ norm_long_kernel(const NormArgs a) {
         for (unsigned long long j = a.cols + threadIdx.x; j < a.pitch; j += blockDim.x) a.q[row * a.pitch + j] = 0;
 }
 
-// Floats a CTA of 1024 threads keeps in registers (32 a thread).
-constexpr unsigned kNormRegCols = 32768;
+// Row lengths that a CTA of 1024 threads keeps in registers: nine groups a
+// thread forward, four of two tensors backward.
+constexpr unsigned kNormRegCols = 32768, kNormBwdRegCols = 16384;
+bool fits(unsigned cols, unsigned most, bool skewed) { return cols <= (skewed ? most - 3 : most); }
 
-template <int MODE, int VEC, int NV>
-void launch_norm_nv(const NormArgs& a, unsigned T, unsigned R) {
-    const unsigned long long ctas = (a.rows + R - 1) / R;
+// Threads a row: four groups each, so that a thread has enough loads in flight,
+// or one each where the rows are fewer than the SMs and latency counts.
+struct RowShape {
+    unsigned threads, rows, per;  // threads a row, rows a CTA, groups a thread
+};
+RowShape row_shape(unsigned cols, bool skewed, std::size_t rows) {
+    const unsigned groups = skewed ? (cols + 3 + 3) / 4 : cols / 4;
+    const unsigned want = rows <= static_cast<unsigned>(sm_count()) ? 1 : 4;
+    RowShape s{};
+    s.threads = std::min(1024u, ((groups + want - 1) / want + 31) / 32 * 32);
+    s.rows = s.threads == 32 ? 8 : 1;
+    s.per = (groups + s.threads - 1) / s.threads;
+    return s;
+}
+
+// Whether rows `stride` floats apart from p lie on the 16-byte grid.
+bool on_grid(const float* p, std::size_t stride, std::size_t rows) {
+    return !p || (aligned16(p) && (rows == 1 || stride % 4 == 0));
+}
+// Whether both tensors' rows have the same skew, row by row.
+bool same_skew(const float* p, std::size_t ps, const float* q, std::size_t qs, std::size_t rows) {
+    return !q || ((reinterpret_cast<std::uintptr_t>(p) & 15) == (reinterpret_cast<std::uintptr_t>(q) & 15) &&
+                  (rows == 1 || ps % 4 == qs % 4));
+}
+
+template <int MODE, bool SKEWED, int NV>
+void launch_norm_nv(const NormArgs& a, const RowShape& s) {
+    const unsigned long long ctas = (a.rows + s.rows - 1) / s.rows;
     if (ctas > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm: too many rows");
-    norm_kernel<MODE, VEC, NV><<<static_cast<unsigned>(ctas), dim3(T, R), 0, stream()>>>(a);
+    norm_kernel<MODE, SKEWED, NV><<<static_cast<unsigned>(ctas), dim3(s.threads, s.rows), 0, stream()>>>(a);
     check_launch("norm_kernel");
+}
+template <int MODE, bool SKEWED>
+void launch_norm_skew(const NormArgs& a) {
+    const RowShape s = row_shape(a.cols, SKEWED, a.rows);
+    if (s.per <= 1) launch_norm_nv<MODE, SKEWED, 1>(a, s);
+    else if (s.per <= 4) launch_norm_nv<MODE, SKEWED, 4>(a, s);
+    else launch_norm_nv<MODE, SKEWED, 9>(a, s);
 }
 
 template <int MODE>
 void launch_norm(const NormArgs& a) {
-    if (a.cols > kNormRegCols) {
+    const bool alike = same_skew(a.x, a.xs, a.r, a.rs, a.rows) && same_skew(a.x, a.xs, a.h, a.cols, a.rows) &&
+                       same_skew(a.x, a.xs, a.y, a.cols, a.rows);
+    const bool skewed = a.cols % 4 != 0 || !on_grid(a.x, a.xs, a.rows) || (a.w && !aligned16(a.w));
+    if (!fits(a.cols, kNormRegCols, skewed) || !alike) {
         if (a.rows > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm: too many rows");
-        norm_long_kernel<MODE><<<static_cast<unsigned>(a.rows), 1024, 0, stream()>>>(a);
+        norm_long_kernel<MODE><<<static_cast<unsigned>(a.rows), std::min(1024u, (a.cols + 31) / 32 * 32), 0, stream()>>>(a);
         check_launch("norm_long_kernel");
         return;
     }
-    const bool vec = a.cols % 4 == 0 && aligned16(a.x) && (a.rows == 1 || a.xs % 4 == 0) &&
-                     (!a.r || (aligned16(a.r) && (a.rows == 1 || a.rs % 4 == 0))) && (!a.w || aligned16(a.w)) &&
-                     (!a.h || aligned16(a.h)) && (!a.y || aligned16(a.y));
-    const unsigned groups = vec ? a.cols / 4 : a.cols;
-    const unsigned per = vec ? 4 : 8;  // groups a thread, while 1024 threads are enough
-    unsigned T = std::min(1024u, ((groups + per - 1) / per + 31) / 32 * 32);
-    const unsigned R = T == 32 ? 8 : 1;
-    const unsigned nv = (groups + T - 1) / T;
-    if (vec) {
-        if (nv <= 4) launch_norm_nv<MODE, 4, 4>(a, T, R);
-        else launch_norm_nv<MODE, 4, 8>(a, T, R);
-    } else {
-        if (nv <= 8) launch_norm_nv<MODE, 1, 8>(a, T, R);
-        else launch_norm_nv<MODE, 1, 32>(a, T, R);
-    }
+    if (skewed) launch_norm_skew<MODE, true>(a);
+    else launch_norm_skew<MODE, false>(a);
 }
 
 // ---- backward -----------------------------------------------------------------
@@ -303,8 +379,63 @@ struct NormBwdArgs {
     float* dh;
 };
 
-__global__ void __launch_bounds__(256)
+// dh, one row a CTA (or a warp) as in the forward: h and t = gy * w stay in
+// registers.
+template <bool SKEWED, int NV>
+__global__ void __launch_bounds__(1024)
 norm_bwd_dh(const NormBwdArgs a) {
+    __shared__ double ssum[32];
+    __shared__ float unused[32];
+    const unsigned long long row = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
+    if (row >= a.rows) return;
+    const unsigned T = blockDim.x, t = threadIdx.x;
+    const float* hp = a.h + row * a.cols;
+    const float* gp = a.gy + row * a.cols;
+    const Span span{SKEWED ? skew_of(hp) : 0, a.cols};
+    const unsigned G = span.groups();
+    const float s = a.rstd[row];
+    Group h[NV], g[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const unsigned at = t + i * T;
+        h[i] = at < G ? load_group<SKEWED>(hp, at, span) : Group{};
+        g[i] = at < G ? load_group<SKEWED>(gp, at, span) : Group{};
+    }
+    double dot = 0.0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const unsigned at = t + i * T;
+        if (at < G) {
+            const Group w = load_weight<SKEWED>(a.w, at, span);
+            float part = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                g[i].v[e] *= w.v[e];
+                part = fmaf(g[i].v[e], h[i].v[e], part);
+            }
+            dot += part;
+        }
+    }
+    dot = reduce_row<NORM_F32>(dot, 0.0f, ssum, unused).sq;
+    const float c = static_cast<float>(dot / a.cols) * (s * s);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const unsigned at = t + i * T;
+        if (at < G) {
+            const Group up = a.gh ? load_group<SKEWED>(a.gh + row * a.cols, at, span) : Group{};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float v = s * (g[i].v[e] - h[i].v[e] * c);
+                g[i].v[e] = a.gh ? v + up.v[e] : v;
+            }
+            store_group<SKEWED>(a.dh + row * a.cols, at, g[i], span);
+        }
+    }
+}
+
+// The same for rows too long for registers, or tensors of unlike alignment.
+__global__ void __launch_bounds__(1024)
+norm_bwd_dh_long(const NormBwdArgs a) {
     __shared__ double scratch[32];
     const unsigned long long at = static_cast<unsigned long long>(blockIdx.x) * a.cols;
     double dot = 0.0;
@@ -319,13 +450,48 @@ norm_bwd_dh(const NormBwdArgs a) {
     }
 }
 
-__global__ void __launch_bounds__(256)
-norm_bwd_dw(const NormBwdArgs a, float* __restrict__ dw) {
+// dw over segments of kDwRows rows, a column a thread, added in float; the
+// segments are then added in double.
+constexpr unsigned kDwRows = 64;
+
+__global__ void __launch_bounds__(128)
+norm_bwd_dw(const NormBwdArgs a, float* __restrict__ partial) {
     const unsigned j = blockIdx.x * blockDim.x + threadIdx.x;
     if (j >= a.cols) return;
-    double s = 0.0;
-    for (unsigned long long i = 0; i < a.rows; ++i) s += a.gy[i * a.cols + j] * (a.h[i * a.cols + j] * a.rstd[i]);
-    dw[j] = static_cast<float>(s);
+    const unsigned long long first = static_cast<unsigned long long>(blockIdx.y) * kDwRows;
+    const unsigned rows = static_cast<unsigned>(min(static_cast<unsigned long long>(kDwRows), a.rows - first));
+    const float* gy = a.gy + first * a.cols + j;
+    const float* h = a.h + first * a.cols + j;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (unsigned i = 0; i < rows; ++i)
+        sum += gy[static_cast<unsigned long long>(i) * a.cols] *
+               (h[static_cast<unsigned long long>(i) * a.cols] * __ldg(a.rstd + first + i));
+    partial[static_cast<unsigned long long>(blockIdx.y) * a.cols + j] = sum;
+}
+
+template <bool SKEWED>
+void launch_dh(const NormBwdArgs& a) {
+    const RowShape s = row_shape(a.cols, SKEWED, a.rows);
+    const unsigned long long ctas = (a.rows + s.rows - 1) / s.rows;
+    const dim3 block(s.threads, s.rows);
+    const unsigned grid = static_cast<unsigned>(ctas);
+    if (s.per <= 1) norm_bwd_dh<SKEWED, 1><<<grid, block, 0, stream()>>>(a);
+    else norm_bwd_dh<SKEWED, 4><<<grid, block, 0, stream()>>>(a);
+    check_launch("norm_bwd_dh");
+}
+
+void launch_dw(const NormBwdArgs& a, float* dw) {
+    const unsigned long long segments = (a.rows + kDwRows - 1) / kDwRows;
+    if (segments > 65535) fail(VC_ERR_OVERFLOW, "rms_norm_backward: too many rows");
+    Scratch partial(segments * a.cols * sizeof(float));
+    norm_bwd_dw<<<dim3((a.cols + 127) / 128, static_cast<unsigned>(segments)), 128, 0, stream()>>>(
+        a, segments > 1 ? partial.as<float>() : dw);
+    check_launch("norm_bwd_dw");
+    if (segments > 1) {
+        const vc_status st = vc_cuda_reduce_axis(VC_REDUCE_SUM, partial.as<float>(), 1, segments, a.cols, dw, nullptr);
+        if (st != VC_OK) fail(st, vc_cuda_last_error());
+    }
 }
 
 void check_rows_cols(const char* what, std::size_t rows, std::size_t cols) {
@@ -416,13 +582,19 @@ vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const f
     if (!dh && !dw) return VC_OK;
     if (rows > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm_backward: too many rows");
     NormBwdArgs a{h, weight, rstd, gy, gh, rows, static_cast<unsigned>(cols), dh};
-    if (dw) {
-        norm_bwd_dw<<<static_cast<unsigned>((cols + 255) / 256), 256, 0, stream()>>>(a, dw);
-        check_launch("norm_bwd_dw");
-    }
+    if (dw) launch_dw(a, dw);
     if (dh) {
-        norm_bwd_dh<<<static_cast<unsigned>(rows), 256, 0, stream()>>>(a);
-        check_launch("norm_bwd_dh");
+        const bool alike = same_skew(h, cols, gy, cols, rows) && same_skew(h, cols, gh, cols, rows) &&
+                           same_skew(h, cols, dh, cols, rows);
+        const bool skewed = cols % 4 != 0 || !aligned16(h) || !aligned16(weight);
+        if (!fits(a.cols, kNormBwdRegCols, skewed) || !alike) {
+            norm_bwd_dh_long<<<static_cast<unsigned>(rows), 1024, 0, stream()>>>(a);
+            check_launch("norm_bwd_dh_long");
+        } else if (skewed) {
+            launch_dh<true>(a);
+        } else {
+            launch_dh<false>(a);
+        }
     }
     VC_API_END
 }
