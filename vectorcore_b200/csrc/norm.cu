@@ -450,6 +450,35 @@ norm_bwd_dh_long(const NormBwdArgs a) {
     }
 }
 
+// dw from `count` partial rows, added in double: 32 columns a CTA, a slice of the
+// rows a warp, the slices added in order. Launched while the kernel that writes
+// the partial rows still runs (the two-launch axis reduction took 15 us here,
+// this takes 4).
+__global__ void __launch_bounds__(1024)
+norm_dw_finish(const float* __restrict__ partial, unsigned long long count, unsigned cols, float* __restrict__ dw) {
+    __shared__ double part[32][33];
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5, j = blockIdx.x * 32 + lane;
+    const unsigned long long per = (count + 31) / 32, first = warp * per, last = min(count, first + per);
+    pdl_wait();
+    double sum = 0.0;
+    if (j < cols) {
+#pragma unroll 8
+        for (unsigned long long i = first; i < last; ++i) sum += partial[i * cols + j];
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && j < cols) {
+        sum = 0.0;
+        for (unsigned v = 0; v < 32; ++v) sum += part[v][lane];
+        dw[j] = static_cast<float>(sum);
+    }
+}
+
+void launch_dw_finish(const float* partial, unsigned long long count, unsigned cols, float* dw) {
+    launch_pdl(norm_dw_finish, dim3((cols + 31) / 32), dim3(1024), 0, stream(), partial, count, cols, dw);
+    check_launch("norm_dw_finish");
+}
+
 // dw over segments of kDwRows rows, a column a thread, added in float; the
 // segments are then added in double.
 constexpr unsigned kDwRows = 64;
@@ -470,6 +499,236 @@ norm_bwd_dw(const NormBwdArgs a, float* __restrict__ partial) {
     partial[static_cast<unsigned long long>(blockIdx.y) * a.cols + j] = sum;
 }
 
+// dh and dw from one pass over h, gy and gh, for aligned rows of up to
+// kRingCols floats: 16 B an element is all that moves. One CTA an SM walks
+// blocks of R rows (R groups of T threads, T * R = kRingThreads). A producer
+// warp bulk-copies the blocks of h and gy into a ring of shared-memory stages;
+// gh is loaded a block ahead into registers. A group adds up the dot product of
+// its next row before it writes dh of its current one, so that the one barrier a
+// row and the sums' latency lie behind work that does not depend on them (the
+// same ring without that, a row at a time: 232 us for 8192 x 8192). A thread
+// owns the same columns in every row, so dw adds up in its registers; the
+// groups' dw meet in shared memory and leave as one partial row a CTA, and the
+// partial rows are added in double.
+constexpr unsigned kRingThreads = 512;
+constexpr unsigned kRingWarps = kRingThreads / 32;
+constexpr unsigned kRingCols = 8192;  // three stages of two rows fit an SM
+constexpr unsigned kRingSmem = 3 * 2 * kRingCols * sizeof(float);
+constexpr unsigned kRingMaxStages = 8;
+
+struct RingArgs {
+    NormBwdArgs n;
+    unsigned T, R;          // threads a row, rows a block
+    unsigned stages;
+    unsigned long long blocks;
+    unsigned segments;      // of kDwRows blocks, the CTA with the most
+    float* partial;         // [grid][segments - 1][R][cols], then [grid][cols]
+    unsigned* err;
+};
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned bytes, unsigned long long* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_addr(dst)),
+                 "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+template <int NV>
+__global__ void __launch_bounds__(kRingThreads + 32, 1)
+norm_bwd_ring(const RingArgs a) {
+    extern __shared__ __align__(128) float ring[];
+    __shared__ unsigned long long full[kRingMaxStages], empty[kRingMaxStages];
+    __shared__ double slots[3][kRingWarps];
+    __shared__ unsigned dead_flag;
+    volatile unsigned* dead = &dead_flag;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned cols = a.n.cols, block_floats = a.R * cols;
+    const unsigned stage_floats = 2 * block_floats;
+    if (threadIdx.x == 0) {
+        dead_flag = 0;
+        for (unsigned s = 0; s < a.stages; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, kRingWarps);
+        }
+        mbar_fence_init();
+    }
+    __syncthreads();
+
+    if (warp == kRingWarps) {  // producer
+        if (lane == 0) {
+            unsigned issued = 0;
+            for (unsigned long long b = blockIdx.x; b < a.blocks; b += gridDim.x, ++issued) {
+                const unsigned slot = issued % a.stages, turn = issued / a.stages;
+                if (turn && (*dead || !mbar_wait_bounded(empty + slot, (turn - 1) & 1, a.err, kWaitPolls / 8))) {
+                    *dead = 1;
+                    break;
+                }
+                const unsigned long long row = b * a.R;
+                const unsigned rows = static_cast<unsigned>(min(static_cast<unsigned long long>(a.R), a.n.rows - row));
+                const unsigned bytes = rows * cols * sizeof(float);
+                float* at = ring + slot * stage_floats;
+                mbar_expect_tx(full + slot, 2 * bytes);
+                bulk_copy(at, a.n.h + row * cols, bytes, full + slot);
+                bulk_copy(at + block_floats, a.n.gy + row * cols, bytes, full + slot);
+            }
+            // the copies still in flight land before the CTA may finish
+            for (unsigned s = issued > a.stages ? issued - a.stages : 0; s < issued; ++s)
+                mbar_wait_bounded(full + s % a.stages, (s / a.stages) & 1, a.err, kWaitPolls / 16);
+        }
+    } else {
+        const unsigned group = threadIdx.x / a.T, t = threadIdx.x - group * a.T;
+        const unsigned G = cols / 4;
+        // the weight stays in registers: the ring leaves L1 too little to hold it
+        Group dw[NV], w[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            dw[i] = Group{};
+            w[i] = t + i * a.T < G ? load_weight<false>(a.n.w, t + i * a.T, Span{0, cols}) : Group{};
+        }
+        unsigned segment = 0;
+        const double by_cols = 1.0 / cols;
+        const auto row_of = [&](unsigned long long b) { return b * a.R + group; };
+        Group up[NV];  // gh of the row whose dot product was added up last
+        float s_of = 0.0f;  // and its rstd
+        // The dot product of block b's row, the i-th of this CTA; dw.
+        const auto take = [&](unsigned long long b, unsigned i_th) {
+            const unsigned slot = i_th % a.stages;
+            const unsigned long long row = row_of(b);
+            const bool mine = row < a.n.rows;
+            s_of = mine ? __ldg(a.n.rstd + row) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const unsigned c = t + i * a.T;
+                up[i] = mine && a.n.gh && c < G ? load_group<false>(a.n.gh + row * cols, c, Span{0, cols}) : Group{};
+            }
+            if (!*dead && !mbar_wait_bounded(full + slot, (i_th / a.stages) & 1, a.err, kWaitPolls / 8)) *dead = 1;
+            const float* at = ring + slot * stage_floats + group * cols;
+            double dot = 0.0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const unsigned c = t + i * a.T;
+                if (mine && c < G) {
+                    const Group h = group_of(reinterpret_cast<const float4*>(at)[c]);
+                    const Group g = group_of(reinterpret_cast<const float4*>(at + block_floats)[c]);
+                    float part = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        dw[i].v[e] = fmaf(g.v[e], h.v[e] * s_of, dw[i].v[e]);
+                        part = fmaf(g.v[e] * w[i].v[e], h.v[e], part);
+                    }
+                    dot += part;
+                }
+            }
+            dot = warp_sum(dot);
+            if (lane == 0) slots[i_th % 3][warp] = dot;
+        };
+        // dh of block b's row, whose gh and rstd are given.
+        const auto give = [&](unsigned long long b, unsigned i_th, const Group (&gh)[NV], float s) {
+            const unsigned slot = i_th % a.stages;
+            const unsigned long long row = row_of(b);
+            const double dot = warp_sum(lane < a.T >> 5 ? slots[i_th % 3][group * (a.T >> 5) + lane] : 0.0);
+            const float c = static_cast<float>(dot * by_cols) * (s * s);
+            if (row < a.n.rows) {
+                const float* at = ring + slot * stage_floats + group * cols;
+                float4* dh = reinterpret_cast<float4*>(a.n.dh + row * cols);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const unsigned at_c = t + i * a.T;
+                    if (at_c >= G) continue;
+                    const Group h = group_of(reinterpret_cast<const float4*>(at)[at_c]);
+                    const Group g = group_of(reinterpret_cast<const float4*>(at + block_floats)[at_c]);
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(s, fmaf(-h.v[e], c, g.v[e] * w[i].v[e]), gh[i].v[e]);
+                    __stcs(dh + at_c, make_float4(o[0], o[1], o[2], o[3]));
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + slot);
+        };
+        unsigned used = 0;
+        if (blockIdx.x < a.blocks) take(blockIdx.x, 0);
+        for (unsigned long long b = blockIdx.x; b < a.blocks; b += gridDim.x, ++used) {
+            Group gh[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) gh[i] = up[i];
+            const float s = s_of;
+            if ((used + 1) % kDwRows == 0 && segment + 1 < a.segments) {  // enough float additions
+                float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const unsigned at_c = t + i * a.T;
+                    if (at_c < G)
+                        reinterpret_cast<float4*>(out)[at_c] = make_float4(dw[i].v[0], dw[i].v[1], dw[i].v[2], dw[i].v[3]);
+                    dw[i] = Group{};
+                }
+                ++segment;
+            }
+            if (b + gridDim.x < a.blocks) take(b + gridDim.x, used + 1);
+            if (a.T > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(a.T) : "memory");
+            else __syncwarp();
+            give(b, used, gh, s);
+        }
+        for (; segment + 1 < a.segments; ++segment) {  // CTAs with fewer blocks
+            float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (t + i * a.T < G) reinterpret_cast<float4*>(out)[t + i * a.T] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        // the groups' rows meet in the ring, which nothing reads any more
+        asm volatile("bar.sync 15, %0;" ::"n"(kRingThreads) : "memory");
+        float4* rows = reinterpret_cast<float4*>(ring);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (t + i * a.T < G)
+                rows[group * G + t + i * a.T] = make_float4(dw[i].v[0], dw[i].v[1], dw[i].v[2], dw[i].v[3]);
+        asm volatile("bar.sync 15, %0;" ::"n"(kRingThreads) : "memory");
+        float4* out = reinterpret_cast<float4*>(a.partial + (static_cast<unsigned long long>(gridDim.x) * (a.segments - 1) * a.R + blockIdx.x) * cols);
+        for (unsigned c = threadIdx.x; c < G; c += kRingThreads) {
+            float4 sum = rows[c];
+            for (unsigned r = 1; r < a.R; ++r) {
+                const float4 v = rows[r * G + c];
+                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            out[c] = sum;
+        }
+    }
+}
+
+// The fused pass, where it applies; false, having launched nothing, otherwise.
+bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
+    if (n.cols % 4 != 0 || n.cols > kRingCols || !aligned16(n.h) || !aligned16(n.gy) || !aligned16(n.w) ||
+        !aligned16(n.dh) || (n.gh && !aligned16(n.gh)))
+        return false;
+    RingArgs a{};
+    a.n = n;
+    a.T = 32;
+    while (a.T < kRingThreads && a.T * 16 < n.cols) a.T *= 2;  // up to four groups a thread
+    a.R = kRingThreads / a.T;
+    a.blocks = (n.rows + a.R - 1) / a.R;
+    const unsigned sms = static_cast<unsigned>(sm_count());
+    if (a.blocks < 3ull * sms) return false;
+    const unsigned stage = 2 * a.R * n.cols * sizeof(float);
+    a.stages = std::min(kRingMaxStages, kRingSmem / stage);
+    const unsigned long long most = (a.blocks + sms - 1) / sms;
+    a.segments = static_cast<unsigned>((most + kDwRows - 1) / kDwRows);
+    const unsigned long long partial_rows = static_cast<unsigned long long>(sms) * ((a.segments - 1) * a.R + 1);
+    Scratch partial(partial_rows * n.cols * sizeof(float));
+    a.partial = partial.as<float>();
+    a.err = device_error_word();
+    const auto launch = [&](auto kernel) {
+        VC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
+        kernel<<<sms, kRingThreads + 32, a.stages * stage, stream()>>>(a);
+    };
+    const unsigned per = (n.cols / 4 + a.T - 1) / a.T;
+    if (per <= 1) launch(norm_bwd_ring<1>);
+    else if (per <= 2) launch(norm_bwd_ring<2>);
+    else launch(norm_bwd_ring<4>);
+    check_launch("norm_bwd_ring");
+    launch_dw_finish(a.partial, partial_rows, n.cols, dw);
+    return true;
+}
+
 template <bool SKEWED>
 void launch_dh(const NormBwdArgs& a) {
     const RowShape s = row_shape(a.cols, SKEWED, a.rows);
@@ -488,10 +747,7 @@ void launch_dw(const NormBwdArgs& a, float* dw) {
     norm_bwd_dw<<<dim3((a.cols + 127) / 128, static_cast<unsigned>(segments)), 128, 0, stream()>>>(
         a, segments > 1 ? partial.as<float>() : dw);
     check_launch("norm_bwd_dw");
-    if (segments > 1) {
-        const vc_status st = vc_cuda_reduce_axis(VC_REDUCE_SUM, partial.as<float>(), 1, segments, a.cols, dw, nullptr);
-        if (st != VC_OK) fail(st, vc_cuda_last_error());
-    }
+    if (segments > 1) launch_dw_finish(partial.as<float>(), segments, a.cols, dw);
 }
 
 void check_rows_cols(const char* what, std::size_t rows, std::size_t cols) {
@@ -582,6 +838,7 @@ vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const f
     if (!dh && !dw) return VC_OK;
     if (rows > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm_backward: too many rows");
     NormBwdArgs a{h, weight, rstd, gy, gh, rows, static_cast<unsigned>(cols), dh};
+    if (dh && dw && try_bwd_ring(a, dw)) return VC_OK;
     if (dw) launch_dw(a, dw);
     if (dh) {
         const bool alike = same_skew(h, cols, gy, cols, rows) && same_skew(h, cols, gh, cols, rows) &&
