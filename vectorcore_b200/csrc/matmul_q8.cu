@@ -33,14 +33,14 @@ struct MatmulQ8Args {
 // One CTA an SM walks the tiles: a warp fetches 128-byte slices of k of both
 // sides by TMA (128-byte swizzle, zeros past the ends, so k, m and n need no
 // alignment), one thread of another issues the products (32 bytes of k each),
-// and four warps scale and store the previous tile out of the other half of
+// and eight warps scale and store the previous tile out of the other half of
 // TMEM meanwhile.
 
 constexpr unsigned kTileM = 128;   // weight rows a tile: TMEM's lanes
 constexpr unsigned kSliceK = 128;  // bytes of k a stage: one swizzled row
 constexpr unsigned kMmaK = 32;     // bytes of k an instruction
-constexpr unsigned kTcThreads = 192;
-constexpr long long kTcPolls = 1ll << 18;  // a wait gives up after about half a second
+constexpr unsigned kStoreWarps = 8;  // two for each quarter of TMEM's lanes
+constexpr unsigned kTcThreads = (kStoreWarps + 2) * 32;
 
 struct TcArgs {
     const float* sa;
@@ -49,7 +49,7 @@ struct TcArgs {
     float* out;
     unsigned m, n;
     unsigned bn;          // tokens a tile, a multiple of 16
-    unsigned slices;      // of k
+    unsigned steps;       // along k: stages a tile takes
     unsigned tiles_m;     // along the tokens
     unsigned tiles_n;     // along the weights
     unsigned stages;
@@ -94,16 +94,45 @@ __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::l
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A bounded wait that also ends when another role of the CTA gave up.
+// A bounded wait that also ends when another role of the CTA gave up. The
+// issuing thread polls without the other kernels' hint to sleep in a poll: waking
+// up cost it 3% of the whole product. The others sleep, which leaves the power
+// (the limit of a long run) to the products.
+constexpr long long kTcPolls = 1ll << 18;  // of up to kWaitHintNs
+template <bool SLEEP = true>
 __device__ __forceinline__ bool tc_wait(unsigned long long* bar, unsigned parity, volatile unsigned* dead,
                                         unsigned* err) {
-    for (long long i = 0; i < kTcPolls; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+    for (long long i = 0; i < (SLEEP ? kTcPolls : kTcPolls << 4); ++i) {
+        if constexpr (SLEEP) {
+            if (mbar_try_wait(bar, parity)) return true;
+        } else {
+            unsigned ok;
+            asm volatile(
+                "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                : "=r"(ok)
+                : "r"(smem_addr(bar)), "r"(parity)
+                : "memory");
+            if (ok) return true;
+        }
         if (*dead) return false;
     }
     *dead = 1;
     atomicOr(err, kErrWaitTimeout);
     return false;
+}
+
+// A place in the ring of stages, and the parity of its current turn.
+struct Place {
+    unsigned slot{0}, parity{0};
+    __device__ __forceinline__ void next(unsigned stages) {
+        if (++slot == stages) slot = 0, parity ^= 1;
+    }
+};
+
+// The copies still in flight land before their CTA may finish.
+__device__ __forceinline__ void drain(unsigned long long* full, unsigned issued, const TcArgs& g) {
+    for (unsigned s = issued > g.stages ? issued - g.stages : 0; s < issued; ++s)
+        mbar_wait_bounded(full + s % g.stages, (s / g.stages) & 1, g.err, kTcPolls);
 }
 
 // Tiles in order: runs of kGroup tiles along the weights for each tile of
@@ -116,6 +145,49 @@ __device__ __forceinline__ void tile_at(unsigned i, const TcArgs& g, unsigned& t
     tn = band * kGroup + in - tm * width;
 }
 
+// A warp's share of a finished tile: 32 weight rows (TMEM lanes, `first` the
+// lowest) and every other 16 tokens, scaled and stored, 128 bytes of one token at
+// a time. The next 16 leave TMEM while the present ones are stored.
+__device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsigned first, unsigned row0) {
+    const unsigned warp = threadIdx.x >> 5, col = first + (threadIdx.x & 31);
+    const bool mine = col < g.n;
+    const float sb = mine ? g.sb[col] : 0.0f, bias = mine && g.bias ? g.bias[col] : 0.0f;
+    const unsigned rows = min(g.bn, g.m - row0), step = 16 * (kStoreWarps / 4);
+    const unsigned taddr = tmem + ((warp & 3) * 32 << 16);
+    const float* sa = g.sa + row0;
+    const bool wide = (reinterpret_cast<std::uintptr_t>(sa) & 15) == 0;
+    unsigned c = 16 * (warp >> 2);
+    int v[16];
+    __syncwarp();
+    if (c < rows) tmem_load16(taddr + c, v);
+    for (; c < rows; c += step) {
+        float s[16];
+        if (wide && c + 16 <= rows) {
+#pragma unroll
+            for (unsigned j = 0; j < 4; ++j) {
+                const float4 f = __ldg(reinterpret_cast<const float4*>(sa + c) + j);
+                s[4 * j] = f.x, s[4 * j + 1] = f.y, s[4 * j + 2] = f.z, s[4 * j + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j) s[j] = c + j < rows ? __ldg(sa + c + j) : 0.0f;
+        }
+        tmem_load_wait();
+#pragma unroll
+        for (unsigned j = 0; j < 16; ++j) s[j] = static_cast<float>(v[j]) * (s[j] * sb);
+        __syncwarp();
+        if (c + step < rows) tmem_load16(taddr + c + step, v);
+        float* out = g.out + static_cast<unsigned long long>(row0 + c) * g.n + col;
+        if (mine) {
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j) {
+                if (c + j < rows) *out = g.bias ? s[j] + bias : s[j];
+                out += g.n;
+            }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kTcThreads, 1)
 matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const TcArgs g) {
     extern __shared__ unsigned char smem_raw[];
@@ -124,7 +196,8 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
     __shared__ unsigned tmem_base, dead_flag;
     volatile unsigned* dead = &dead_flag;
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned stage_bytes = (kTileM + g.bn) * kSliceK;
+    constexpr unsigned a_at = kTileM * kSliceK;
+    const unsigned stage_bytes = a_at + g.bn * kSliceK;
     const unsigned ntiles = g.tiles_m * g.tiles_n;
     if (threadIdx.x == 0) {
         dead_flag = 0;
@@ -134,11 +207,11 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
         }
         for (unsigned s = 0; s < 2; ++s) {
             mbar_init(acc_full + s, 1);
-            mbar_init(acc_empty + s, 4);
+            mbar_init(acc_empty + s, kStoreWarps);
         }
         mbar_fence_init();
     }
-    if (warp == 5)
+    if (warp == kStoreWarps + 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
                      "r"(g.tmem_cols)
                      : "memory");
@@ -147,45 +220,43 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
     tc_fence_after();
     const unsigned tmem = tmem_base;
 
-    if (warp == 4) {  // fetch
+    if (warp == kStoreWarps) {  // fetch
         if (lane == 0) {
+            Place at;
             unsigned issued = 0;
             bool ok = true;
             for (unsigned i = blockIdx.x; ok && i < ntiles; i += gridDim.x) {
                 unsigned tn, tm;
                 tile_at(i, g, tn, tm);
-                for (unsigned s = 0; s < g.slices; ++s, ++issued) {
-                    const unsigned slot = issued % g.stages, turn = issued / g.stages;
-                    if (turn && !(ok = tc_wait(empty + slot, (turn - 1) & 1, dead, g.err))) break;
-                    unsigned char* at = tiles + slot * stage_bytes;
-                    mbar_expect_tx(full + slot, stage_bytes);
-                    tma_load_2d(at, &bmap, full + slot, static_cast<int>(s * kSliceK), static_cast<int>(tn * kTileM));
-                    tma_load_2d(at + kTileM * kSliceK, &amap, full + slot, static_cast<int>(s * kSliceK),
-                                static_cast<int>(tm * g.bn));
+                for (unsigned s = 0; s < g.steps; ++s, ++issued, at.next(g.stages)) {
+                    unsigned long long* bar = full + at.slot;
+                    if (issued >= g.stages && !(ok = tc_wait<false>(empty + at.slot, at.parity ^ 1, dead, g.err))) break;
+                    unsigned char* dst = tiles + at.slot * stage_bytes;
+                    mbar_expect_tx(bar, stage_bytes);
+                    const int x = static_cast<int>(s * kSliceK);
+                    tma_load_2d(dst, &bmap, bar, x, static_cast<int>(tn * kTileM));
+                    tma_load_2d(dst + a_at, &amap, bar, x, static_cast<int>(tm * g.bn));
                 }
             }
-            // the copies still in flight land before the CTA may finish
-            for (unsigned s = issued > g.stages ? issued - g.stages : 0; s < issued; ++s)
-                mbar_wait_bounded(full + s % g.stages, (s / g.stages) & 1, g.err, kTcPolls);
+            drain(full, issued, g);
         }
-    } else if (warp == 5) {  // products
+    } else if (warp == kStoreWarps + 1) {  // products
         if (lane == 0) {
-            unsigned used = 0, turn = 0;
+            Place at;
+            unsigned turn = 0;
             bool ok = true;
+            const unsigned long long da0 = tile_desc(smem_addr(tiles)), db0 = da0 + (a_at >> 4);
             for (unsigned i = blockIdx.x; ok && i < ntiles; i += gridDim.x, ++turn) {
-                const unsigned half = turn & 1;
-                if (turn > 1 && !(ok = tc_wait(acc_empty + half, ((turn >> 1) - 1) & 1, dead, g.err))) break;
+                const unsigned half = turn & 1, d = tmem + half * g.bn;
+                if (turn > 1 && !(ok = tc_wait<false>(acc_empty + half, ((turn >> 1) - 1) & 1, dead, g.err))) break;
                 tc_fence_after();
-                for (unsigned s = 0; s < g.slices; ++s, ++used) {
-                    const unsigned slot = used % g.stages;
-                    if (!(ok = tc_wait(full + slot, (used / g.stages) & 1, dead, g.err))) break;
-                    tc_fence_after();
-                    const unsigned at = smem_addr(tiles + slot * stage_bytes);
-                    const unsigned long long da = tile_desc(at), db = tile_desc(at + kTileM * kSliceK);
+                for (unsigned s = 0; s < g.steps; ++s, at.next(g.stages)) {
+                    if (!(ok = tc_wait<false>(full + at.slot, at.parity, dead, g.err))) break;
+                    const unsigned long long skip = at.slot * (stage_bytes >> 4);
 #pragma unroll
                     for (unsigned j = 0; j < kSliceK / kMmaK; ++j)
-                        mma_i8(tmem + half * g.bn, da + j * (kMmaK >> 4), db + j * (kMmaK >> 4), g.idesc, s + j != 0);
-                    mma_commit(empty + slot);
+                        mma_i8(d, da0 + skip + j * (kMmaK >> 4), db0 + skip + j * (kMmaK >> 4), g.idesc, s + j != 0);
+                    mma_commit(empty + at.slot);
                 }
                 if (ok) mma_commit(acc_full + half);
             }
@@ -198,26 +269,7 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
             tc_fence_after();
             unsigned tn, tm;
             tile_at(i, g, tn, tm);
-            const unsigned col = tn * kTileM + warp * 32 + lane;
-            const bool mine = col < g.n;
-            const float sb = mine ? g.sb[col] : 0.0f, bias = mine && g.bias ? g.bias[col] : 0.0f;
-            const unsigned row0 = tm * g.bn, rows = min(g.bn, g.m - row0);
-            float* out = g.out + static_cast<unsigned long long>(row0) * g.n + col;
-            const unsigned taddr = tmem + (warp * 32 << 16) + half * g.bn;
-            for (unsigned c = 0; c < rows; c += 16) {
-                int v[16];
-                __syncwarp();
-                tmem_load16(taddr + c, v);
-                tmem_load_wait();
-                if (mine) {
-#pragma unroll
-                    for (unsigned j = 0; j < 16; ++j)
-                        if (c + j < rows) {
-                            const float p = static_cast<float>(v[j]) * (__ldg(g.sa + row0 + c + j) * sb);
-                            out[static_cast<unsigned long long>(c + j) * g.n] = g.bias ? p + bias : p;
-                        }
-                }
-            }
+            store_tile(g, tmem + half * g.bn, tn * kTileM + (warp & 3) * 32, tm * g.bn);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty + half);
@@ -226,10 +278,163 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kStoreWarps + 1) {
         tc_fence_after();
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols));
+    }
+}
+
+// The same with pairs of CTAs on one tile of 256 weight rows: each CTA fetches
+// its own 128 weight rows and half of the tokens, and the instruction, issued by
+// the first CTA of the pair, reads both CTAs' shared memory: a third less to
+// fetch and to hold for a stage. A stage holds 256 bytes of k, eight products:
+// with 128 the one thread's wait, issue and commit took longer than the four
+// products they bring (8192^3: 385 us, with 256 324 us).
+constexpr unsigned kPairSlices = 2;
+
+__device__ __forceinline__ unsigned in_cta(const void* p, unsigned rank) {
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, unsigned bar, int x, int y) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_i8_pair(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc,
+                                            bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<unsigned>(accumulate))
+        : "memory");
+}
+// arrives at the barrier of this place in both CTAs
+__device__ __forceinline__ void mma_commit_pair(unsigned long long* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"(static_cast<unsigned short>(3))
+        : "memory");
+}
+__device__ __forceinline__ void arrive_at(unsigned bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kTcThreads, 1)
+matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const TcArgs g) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    __shared__ unsigned long long full[8], empty[8], acc_full[2], acc_empty[2];
+    __shared__ unsigned tmem_base, dead_flag;
+    volatile unsigned* dead = &dead_flag;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = blockIdx.x & 1, pairs = gridDim.x >> 1, first = blockIdx.x >> 1;
+    const unsigned half_bn = g.bn / 2;
+    constexpr unsigned a_at = kPairSlices * kTileM * kSliceK;
+    const unsigned stage_bytes = a_at + kPairSlices * half_bn * kSliceK;
+    const unsigned ntiles = g.tiles_m * g.tiles_n;
+    if (threadIdx.x == 0) {
+        dead_flag = 0;
+        for (unsigned s = 0; s < g.stages; ++s) {
+            mbar_init(full + s, 1);   // the first CTA's are used
+            mbar_init(empty + s, 1);
+        }
+        for (unsigned s = 0; s < 2; ++s) {
+            mbar_init(acc_full + s, 1);
+            mbar_init(acc_empty + s, 2 * kStoreWarps);  // the first CTA's: the warps of both
+        }
+        mbar_fence_init();
+    }
+    if (warp == kStoreWarps + 1)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(g.tmem_cols)
+                     : "memory");
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();
+    tc_fence_after();
+    const unsigned tmem = tmem_base;
+
+    if (warp == kStoreWarps) {  // fetch
+        if (lane == 0) {
+            Place at;
+            unsigned issued = 0;
+            bool ok = true;
+            const unsigned bars = in_cta(full, 0);
+            for (unsigned i = first; ok && i < ntiles; i += pairs) {
+                unsigned tn, tm;
+                tile_at(i, g, tn, tm);
+                const int row_b = static_cast<int>((2 * tn + rank) * kTileM), row_a = static_cast<int>(tm * g.bn + rank * half_bn);
+                for (unsigned s = 0; s < g.steps; ++s, ++issued, at.next(g.stages)) {
+                    if (issued >= g.stages && !(ok = tc_wait<false>(empty + at.slot, at.parity ^ 1, dead, g.err))) break;
+                    unsigned char* dst = tiles + at.slot * stage_bytes;
+                    const unsigned bar = bars + at.slot * 8;
+                    if (rank == 0) mbar_expect_tx(full + at.slot, 2 * stage_bytes);
+                    for (unsigned j = 0; j < kPairSlices; ++j) {
+                        const int x = static_cast<int>((s * kPairSlices + j) * kSliceK);
+                        tma_load_2d_pair(dst + j * kTileM * kSliceK, &bmap, bar, x, row_b);
+                        tma_load_2d_pair(dst + a_at + j * half_bn * kSliceK, &amap, bar, x, row_a);
+                    }
+                }
+            }
+            // the second CTA's copies are waited for by the first (cluster barrier below)
+            if (rank == 0) drain(full, issued, g);
+        }
+    } else if (warp == kStoreWarps + 1) {  // products, issued by the first CTA
+        if (lane == 0 && rank == 0) {
+            Place at;
+            unsigned turn = 0;
+            bool ok = true;
+            const unsigned long long da0 = tile_desc(smem_addr(tiles)), db0 = da0 + (a_at >> 4);
+            for (unsigned i = first; ok && i < ntiles; i += pairs, ++turn) {
+                const unsigned half = turn & 1, d = tmem + half * g.bn;
+                if (turn > 1 && !(ok = tc_wait<false>(acc_empty + half, ((turn >> 1) - 1) & 1, dead, g.err))) break;
+                tc_fence_after();
+                for (unsigned s = 0; s < g.steps; ++s, at.next(g.stages)) {
+                    if (!(ok = tc_wait<false>(full + at.slot, at.parity, dead, g.err))) break;
+                    const unsigned long long skip = at.slot * (stage_bytes >> 4);
+#pragma unroll
+                    for (unsigned p = 0; p < kPairSlices; ++p) {
+                        const unsigned long long da = da0 + skip + p * (kTileM * kSliceK >> 4);
+                        const unsigned long long db = db0 + skip + p * (half_bn * kSliceK >> 4);
+#pragma unroll
+                        for (unsigned j = 0; j < kSliceK / kMmaK; ++j)
+                            mma_i8_pair(d, da + j * (kMmaK >> 4), db + j * (kMmaK >> 4), g.idesc, s + p + j != 0);
+                    }
+                    mma_commit_pair(empty + at.slot);
+                }
+                if (ok) mma_commit_pair(acc_full + half);
+            }
+        }
+    } else {  // scale and store
+        unsigned turn = 0;
+        for (unsigned i = first; i < ntiles; i += pairs, ++turn) {
+            const unsigned half = turn & 1;
+            if (!tc_wait(acc_full + half, (turn >> 1) & 1, dead, g.err)) break;
+            tc_fence_after();
+            unsigned tn, tm;
+            tile_at(i, g, tn, tm);
+            store_tile(g, tmem + half * g.bn, (2 * tn + rank) * kTileM + (warp & 3) * 32, tm * g.bn);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(in_cta(acc_empty + half, 0));
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();  // neither CTA's shared memory is read or arrived at any more
+    if (warp == kStoreWarps + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols));
     }
 }
 
@@ -260,31 +465,47 @@ CUtensorMap slice_map(const signed char* p, unsigned rows, unsigned k, unsigned 
     return map;
 }
 
-void launch_tc(const MatmulQ8Args& a) {
+void launch_tc(const MatmulQ8Args& a, bool pair) {
     TcArgs g{};
     g.sa = a.sa, g.sb = a.sb, g.bias = a.bias, g.out = a.out, g.m = a.m, g.n = a.n;
     g.err = device_error_word();
-    g.bn = std::min(256u, (a.m + 15) / 16 * 16);
-    g.slices = (a.k + kSliceK - 1) / kSliceK;
+    const unsigned step = pair ? 32 : 16;
+    g.bn = std::min(256u, (a.m + step - 1) / step * step);
+    const unsigned slices = pair ? kPairSlices : 1;
+    g.steps = (a.k + slices * kSliceK - 1) / (slices * kSliceK);
+    const unsigned tile_n = pair ? 2 * kTileM : kTileM;
     g.tiles_m = (a.m + g.bn - 1) / g.bn;
-    g.tiles_n = (a.n + kTileM - 1) / kTileM;
-    const unsigned stage = (kTileM + g.bn) * kSliceK;
+    g.tiles_n = (a.n + tile_n - 1) / tile_n;
+    const unsigned tokens = pair ? g.bn / 2 : g.bn;  // a CTA fetches
+    const unsigned stage = slices * (kTileM + tokens) * kSliceK;
     g.stages = std::min(8u, 220u * 1024 / stage);
     g.tmem_cols = 32;
     while (g.tmem_cols < 2 * g.bn) g.tmem_cols *= 2;
     // 32-bit integer accumulators, signed 8-bit sides, both K-major
-    g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (kTileM >> 4) << 24;
+    g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (tile_n >> 4) << 24;
     if (static_cast<unsigned long long>(g.tiles_m) * g.tiles_n > 0x7fffffffull)
         fail(VC_ERR_OVERFLOW, "matmul_q8: too many tiles");
-    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn);
+    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, tokens);
     constexpr unsigned kMaxSmem = 222 * 1024;
     static bool configured = false;
     if (!configured) {
         VC_CUDA(cudaFuncSetAttribute(matmul_q8_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+        VC_CUDA(cudaFuncSetAttribute(matmul_q8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
         configured = true;
     }
-    const unsigned grid = std::min(g.tiles_m * g.tiles_n, static_cast<unsigned>(sm_count()));
-    matmul_q8_tc<<<grid, kTcThreads, g.stages * stage + 1024, stream()>>>(bmap, amap, g);
+    const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(pair ? 2 * std::min(ntiles, sms / 2) : std::min(ntiles, sms));
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = g.stages * stage + 1024;
+    cfg.stream = stream();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pair ? 1 : 0;
+    VC_CUDA(cudaLaunchKernelEx(&cfg, pair ? matmul_q8_pair : matmul_q8_tc, bmap, amap, g));
     check_launch("matmul_q8_tc");
 }
 
@@ -320,7 +541,7 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
         matmul_q8_empty<<<grid_for(m * n, 256), 256, 0, stream()>>>(a_scale, b_scale, bias, g.m, g.n, out);
         check_launch("matmul_q8_empty");
     } else {
-        launch_tc(g);
+        launch_tc(g, m > 128);
     }
     VC_API_END
 }
