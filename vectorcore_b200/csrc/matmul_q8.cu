@@ -23,6 +23,112 @@ struct MatmulQ8Args {
     unsigned m, n, k;
 };
 
+// ---- few tokens -------------------------------------------------------------------
+//
+// Up to 8 * NT tokens: the time is the weights' way from HBM, so nothing stands
+// between them and the registers. A CTA has 16 weight rows, its eight warps take
+// 128-byte pieces of k in turn, 16 bytes a thread and load, and multiply them by
+// m16n8k32 products. A product's four groups of k may be any four as long as both
+// sides agree, so a thread's 16 consecutive bytes serve as they are; no byte is
+// moved between threads. The warps' sums meet in shared memory.
+constexpr unsigned kRowsWarps = 8;
+constexpr unsigned kPiece = 128;  // bytes of k a warp takes at a time
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], int a0, int a1, int a2, int a3, int b0, int b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// weights are read once: not kept in L1
+__device__ __forceinline__ int4 load_weights(const signed char* p) {
+    int4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+// the bytes of a 16-byte group that are below k (`left` of them)
+__device__ __forceinline__ int4 keep_bytes(int4 v, int left) {
+    const auto word = [&](int w, int at) {
+        const int n = left - at;
+        return n >= 4 ? w : n <= 0 ? 0 : static_cast<int>(static_cast<unsigned>(w) & ((1u << (8 * n)) - 1));
+    };
+    return make_int4(word(v.x, 0), word(v.y, 4), word(v.z, 8), word(v.w, 12));
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kRowsWarps * 32)
+matmul_q8_rows(const MatmulQ8Args g) {
+    __shared__ int sums[kRowsWarps][16][8 * NT + 1];
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q = lane & 3;
+    const unsigned row0 = blockIdx.x * 16;
+    const signed char* w0 = g.b + static_cast<unsigned long long>(min(row0 + r, g.n - 1)) * g.bp + q * 16;
+    const signed char* w1 = g.b + static_cast<unsigned long long>(min(row0 + r + 8, g.n - 1)) * g.bp + q * 16;
+    const signed char* x[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) x[i] = g.a + static_cast<unsigned long long>(min(r + 8u * i, g.m - 1)) * g.ap + q * 16;
+    int acc[NT][4] = {};
+    const unsigned whole = g.k / kPiece;
+#pragma unroll 2
+    for (unsigned piece = warp; piece < whole; piece += kRowsWarps) {
+        const unsigned at = piece * kPiece;
+        const int4 a0 = load_weights(w0 + at), a1 = load_weights(w1 + at);
+        const int4 c0 = load_weights(w0 + at + 64), c1 = load_weights(w1 + at + 64);
+        int4 b[NT], d[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            b[i] = __ldg(reinterpret_cast<const int4*>(x[i] + at));
+            d[i] = __ldg(reinterpret_cast<const int4*>(x[i] + at + 64));
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            mma_s8(acc[i], a0.x, a1.x, a0.y, a1.y, b[i].x, b[i].y);
+            mma_s8(acc[i], a0.z, a1.z, a0.w, a1.w, b[i].z, b[i].w);
+            mma_s8(acc[i], c0.x, c1.x, c0.y, c1.y, d[i].x, d[i].y);
+            mma_s8(acc[i], c0.z, c1.z, c0.w, c1.w, d[i].z, d[i].w);
+        }
+    }
+    // what is left of k, less than a piece: 64 bytes a warp; a thread's bytes past
+    // k are dropped from the tokens, whose products are then zero
+    for (unsigned at = whole * kPiece + 64 * warp; at < g.k; at += 64 * kRowsWarps) {
+        const int left = static_cast<int>(g.k) - static_cast<int>(at + q * 16);
+        const int4 none = make_int4(0, 0, 0, 0);
+        const int4 a0 = left > 0 ? load_weights(w0 + at) : none, a1 = left > 0 ? load_weights(w1 + at) : none;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int4 b = left > 0 ? keep_bytes(__ldg(reinterpret_cast<const int4*>(x[i] + at)), left) : none;
+            mma_s8(acc[i], a0.x, a1.x, a0.y, a1.y, b.x, b.y);
+            mma_s8(acc[i], a0.z, a1.z, a0.w, a1.w, b.z, b.w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        sums[warp][r][8 * i + 2 * q] = acc[i][0];
+        sums[warp][r][8 * i + 2 * q + 1] = acc[i][1];
+        sums[warp][r + 8][8 * i + 2 * q] = acc[i][2];
+        sums[warp][r + 8][8 * i + 2 * q + 1] = acc[i][3];
+    }
+    __syncthreads();
+    for (unsigned i = threadIdx.x; i < 16 * 8 * NT; i += kRowsWarps * 32) {
+        const unsigned token = i >> 4, row = i & 15;
+        if (token >= g.m || row0 + row >= g.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (unsigned v = 0; v < kRowsWarps; ++v) sum += sums[v][row][token];
+        const float p = static_cast<float>(sum) * (g.sa[token] * g.sb[row0 + row]);
+        g.out[static_cast<unsigned long long>(token) * g.n + row0 + row] = g.bias ? p + g.bias[row0 + row] : p;
+    }
+}
+
+void launch_rows(const MatmulQ8Args& g) {
+    const unsigned grid = (g.n + 15) / 16;
+    if (g.m <= 8) matmul_q8_rows<1><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
+    else if (g.m <= 16) matmul_q8_rows<2><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
+    else matmul_q8_rows<4><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
+    check_launch("matmul_q8_rows");
+}
+
 // ---- Blackwell tensor cores ------------------------------------------------------
 //
 // The weights b are the instruction's M side and the tokens a its N side, so a
@@ -33,13 +139,13 @@ struct MatmulQ8Args {
 // One CTA an SM walks the tiles: a warp fetches 128-byte slices of k of both
 // sides by TMA (128-byte swizzle, zeros past the ends, so k, m and n need no
 // alignment), one thread of another issues the products (32 bytes of k each),
-// and eight warps scale and store the previous tile out of the other half of
+// and sixteen warps scale and store the previous tile out of the other half of
 // TMEM meanwhile.
 
 constexpr unsigned kTileM = 128;   // weight rows a tile: TMEM's lanes
 constexpr unsigned kSliceK = 128;  // bytes of k a stage: one swizzled row
 constexpr unsigned kMmaK = 32;     // bytes of k an instruction
-constexpr unsigned kStoreWarps = 8;  // two for each quarter of TMEM's lanes
+constexpr unsigned kStoreWarps = 16;  // four for each quarter of TMEM's lanes
 constexpr unsigned kTcThreads = (kStoreWarps + 2) * 32;
 
 struct TcArgs {
@@ -175,15 +281,20 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
         tmem_load_wait();
 #pragma unroll
         for (unsigned j = 0; j < 16; ++j) s[j] = static_cast<float>(v[j]) * (s[j] * sb);
+        if (g.bias) {
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j) s[j] += bias;
+        }
         __syncwarp();
         if (c + step < rows) tmem_load16(taddr + c + step, v);
         float* out = g.out + static_cast<unsigned long long>(row0 + c) * g.n + col;
-        if (mine) {
+        if (mine && c + 16 <= rows) {
 #pragma unroll
-            for (unsigned j = 0; j < 16; ++j) {
-                if (c + j < rows) *out = g.bias ? s[j] + bias : s[j];
-                out += g.n;
-            }
+            for (unsigned j = 0; j < 16; ++j) out[static_cast<unsigned long long>(j) * g.n] = s[j];
+        } else if (mine) {
+#pragma unroll
+            for (unsigned j = 0; j < 16; ++j)
+                if (c + j < rows) out[static_cast<unsigned long long>(j) * g.n] = s[j];
         }
     }
 }
@@ -540,6 +651,8 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
     if (k == 0) {
         matmul_q8_empty<<<grid_for(m * n, 256), 256, 0, stream()>>>(a_scale, b_scale, bias, g.m, g.n, out);
         check_launch("matmul_q8_empty");
+    } else if (m <= 32) {
+        launch_rows(g);
     } else {
         launch_tc(g, m > 128);
     }
