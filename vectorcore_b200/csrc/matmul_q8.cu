@@ -31,6 +31,7 @@ struct MatmulQ8Args {
 // m16n8k32 products. A product's four groups of k may be any four as long as both
 // sides agree, so a thread's 16 consecutive bytes serve as they are; no byte is
 // moved between threads. The warps' sums meet in shared memory.
+constexpr unsigned kRowsTokens = 16;
 constexpr unsigned kRowsWarps = 8;
 constexpr unsigned kPiece = 128;  // bytes of k a warp takes at a time
 
@@ -124,8 +125,7 @@ matmul_q8_rows(const MatmulQ8Args g) {
 void launch_rows(const MatmulQ8Args& g) {
     const unsigned grid = (g.n + 15) / 16;
     if (g.m <= 8) matmul_q8_rows<1><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
-    else if (g.m <= 16) matmul_q8_rows<2><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
-    else matmul_q8_rows<4><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
+    else matmul_q8_rows<2><<<grid, kRowsWarps * 32, 0, stream()>>>(g);
     check_launch("matmul_q8_rows");
 }
 
@@ -139,13 +139,13 @@ void launch_rows(const MatmulQ8Args& g) {
 // One CTA an SM walks the tiles: a warp fetches 128-byte slices of k of both
 // sides by TMA (128-byte swizzle, zeros past the ends, so k, m and n need no
 // alignment), one thread of another issues the products (32 bytes of k each),
-// and sixteen warps scale and store the previous tile out of the other half of
+// and eight warps scale and store the previous tile out of the other half of
 // TMEM meanwhile.
 
 constexpr unsigned kTileM = 128;   // weight rows a tile: TMEM's lanes
 constexpr unsigned kSliceK = 128;  // bytes of k a stage: one swizzled row
 constexpr unsigned kMmaK = 32;     // bytes of k an instruction
-constexpr unsigned kStoreWarps = 16;  // four for each quarter of TMEM's lanes
+constexpr unsigned kStoreWarps = 8;  // two for each quarter of TMEM's lanes
 constexpr unsigned kTcThreads = (kStoreWarps + 2) * 32;
 
 struct TcArgs {
@@ -396,6 +396,156 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
     }
 }
 
+// Too few tiles for the SMs: a cluster of S CTAs shares a tile, each taking its
+// part of k. A CTA hands every other one the sums of a share of the tokens and
+// adds up its own share, which it scales and stores. The sums meet in scratch
+// memory, which stays in L2: the cluster's shared memory takes some 15 bytes a
+// clock from its neighbours, L2 four times that (256 x 4096 x 4096 spent 12 of 21
+// us on the exchange by way of shared memory). One tile a CTA, no double buffer.
+struct SplitArgs {
+    TcArgs g;
+    unsigned split;       // CTAs a tile, a power of two up to 8
+    unsigned part;        // steps along k a CTA
+    int* sums;            // scratch: [tile][CTA of the cluster][token][weight row]
+};
+
+__device__ __forceinline__ unsigned in_cta(const void* p, unsigned rank) {
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(kTcThreads, 1)
+matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const SplitArgs a) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    __shared__ unsigned long long full[8], empty[8], acc_full[1];
+    __shared__ unsigned tmem_base, dead_flag;
+    volatile unsigned* dead = &dead_flag;
+    const TcArgs& g = a.g;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned tile = blockIdx.x / a.split, rank = blockIdx.x - tile * a.split;
+    const unsigned tm = tile / g.tiles_n, tn = tile - tm * g.tiles_n;
+    const unsigned first = rank * a.part, last = min(g.steps, first + a.part);
+    constexpr unsigned a_at = kTileM * kSliceK;
+    const unsigned stage_bytes = a_at + g.bn * kSliceK;
+    const auto fetch = [&](unsigned step, unsigned slot) {
+        unsigned char* dst = tiles + slot * stage_bytes;
+        mbar_expect_tx(full + slot, stage_bytes);
+        const int x = static_cast<int>(step * kSliceK);
+        tma_load_2d(dst, &bmap, full + slot, x, static_cast<int>(tn * kTileM));
+        tma_load_2d(dst + a_at, &amap, full + slot, x, static_cast<int>(tm * g.bn));
+    };
+    const unsigned ahead = min(g.stages, last - first);
+    if (warp == kStoreWarps && lane == 0) {
+        dead_flag = 0;
+        for (unsigned s = 0; s < g.stages; ++s) {
+            mbar_init(full + s, 1);
+            mbar_init(empty + s, 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_fence_init();
+        // the first stages are on their way while the others set up
+        for (unsigned s = 0; s < ahead; ++s) fetch(first + s, s);
+    }
+    if (warp == kStoreWarps + 1)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
+                     "r"(g.tmem_cols)
+                     : "memory");
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_base;
+
+    if (warp == kStoreWarps) {  // fetch
+        if (lane == 0) {
+            unsigned issued = ahead;
+            Place at;
+            for (unsigned s = first + ahead; s < last; ++s, ++issued, at.next(g.stages)) {
+                if (!tc_wait<false>(empty + at.slot, at.parity, dead, g.err)) break;
+                fetch(s, at.slot);
+            }
+            drain(full, issued, g);
+        }
+    } else if (warp == kStoreWarps + 1) {  // products
+        if (lane == 0) {
+            Place at;
+            bool ok = true;
+            const unsigned long long da0 = tile_desc(smem_addr(tiles)), db0 = da0 + (a_at >> 4);
+            for (unsigned s = first; s < last; ++s, at.next(g.stages)) {
+                if (!(ok = tc_wait<false>(full + at.slot, at.parity, dead, g.err))) break;
+                const unsigned long long skip = at.slot * (stage_bytes >> 4);
+#pragma unroll
+                for (unsigned j = 0; j < kSliceK / kMmaK; ++j)
+                    mma_i8(tmem, da0 + skip + j * (kMmaK >> 4), db0 + skip + j * (kMmaK >> 4), g.idesc, s - first + j != 0);
+                mma_commit(empty + at.slot);
+            }
+            if (ok) mma_commit(acc_full);
+        }
+    } else {
+        const bool ok = tc_wait<false>(acc_full, 0, dead, g.err);
+        tc_fence_after();
+        if (ok && a.split == 1) store_tile(g, tmem, tn * kTileM + (warp & 3) * 32, tm * g.bn);
+    }
+    if (a.split > 1) {
+        const unsigned share = g.bn / a.split, mine0 = rank * share;
+        int* sums = a.sums + static_cast<unsigned long long>(tile) * a.split * g.bn * kTileM;  // the tile's
+        const unsigned l = (warp & 3) * 32 + lane, taddr = tmem + ((warp & 3) * 32 << 16);
+        constexpr unsigned stride = 16 * (kStoreWarps / 4);
+        if (warp < kStoreWarps) {
+            // tokens 16 at a time, a lane the sums of one weight row; its own share stays
+            int* own = sums + static_cast<unsigned long long>(rank) * g.bn * kTileM + l;
+            for (unsigned c = 16 * (warp >> 2); c < g.bn; c += stride) {
+                int v[16];
+                tmem_load16(taddr + c, v);
+                tmem_load_wait();
+#pragma unroll
+                for (unsigned j = 0; j < 16; ++j)
+                    if (c + j - mine0 >= share) __stcg(own + (c + j) * kTileM, v[j]);
+            }
+            __threadfence();
+        }
+        __syncwarp();
+        cluster_barrier();
+        if (warp < kStoreWarps) {
+            const unsigned col = tn * kTileM + l;
+            const bool mine = col < g.n;
+            const float sb = mine ? g.sb[col] : 0.0f, bias = mine && g.bias ? g.bias[col] : 0.0f;
+            for (unsigned c = mine0 / 16 * 16 + 16 * (warp >> 2); c < mine0 + share; c += stride) {
+                int v[16];
+                tmem_load16(taddr + c, v);
+                tmem_load_wait();
+                for (unsigned r = 0; r < a.split; ++r) {
+                    if (r == rank) continue;
+                    const int* other = sums + static_cast<unsigned long long>(r) * g.bn * kTileM + l;
+#pragma unroll
+                    for (unsigned j = 0; j < 16; ++j)
+                        if (c + j - mine0 < share) v[j] += __ldcg(other + (c + j) * kTileM);
+                }
+                const unsigned row0 = tm * g.bn + c;
+#pragma unroll
+                for (unsigned j = 0; j < 16; ++j)
+                    if (c + j - mine0 < share && mine && row0 + j < g.m) {
+                        const float p = static_cast<float>(v[j]) * (__ldg(g.sa + row0 + j) * sb);
+                        g.out[static_cast<unsigned long long>(row0 + j) * g.n + col] = g.bias ? p + bias : p;
+                    }
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kStoreWarps + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols));
+    }
+}
+
 // The same with pairs of CTAs on one tile of 256 weight rows: each CTA fetches
 // its own 128 weight rows and half of the tokens, and the instruction, issued by
 // the first CTA of the pair, reads both CTAs' shared memory: a third less to
@@ -404,11 +554,6 @@ matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ C
 // products they bring (8192^3: 385 us, with 256 324 us).
 constexpr unsigned kPairSlices = 2;
 
-__device__ __forceinline__ unsigned in_cta(const void* p, unsigned rank) {
-    unsigned a;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
-    return a;
-}
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, unsigned bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
@@ -434,10 +579,6 @@ __device__ __forceinline__ void mma_commit_pair(unsigned long long* bar) {
 __device__ __forceinline__ void arrive_at(unsigned bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 __global__ void __launch_bounds__(kTcThreads, 1)
 matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const TcArgs g) {
     extern __shared__ unsigned char smem_raw[];
@@ -620,6 +761,53 @@ void launch_tc(const MatmulQ8Args& a, bool pair) {
     check_launch("matmul_q8_tc");
 }
 
+// The least steps along k that are worth a CTA of their own.
+constexpr unsigned kSplitSteps = 4;
+
+void launch_split(const MatmulQ8Args& a) {
+    SplitArgs p{};
+    TcArgs& g = p.g;
+    g.sa = a.sa, g.sb = a.sb, g.bias = a.bias, g.out = a.out, g.m = a.m, g.n = a.n;
+    g.err = device_error_word();
+    const unsigned token_tiles = (a.m + 255) / 256;
+    g.bn = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    g.steps = (a.k + kSliceK - 1) / kSliceK;
+    g.tiles_m = (a.m + g.bn - 1) / g.bn;
+    g.tiles_n = (a.n + kTileM - 1) / kTileM;
+    const unsigned stage = (kTileM + g.bn) * kSliceK;
+    const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
+    g.stages = std::min(8u, 220u * 1024 / stage);
+    p.split = 1;
+    while (p.split < 8 && 2 * p.split * ntiles <= sms && g.steps >= 2 * p.split * kSplitSteps) p.split *= 2;
+    p.part = (g.steps + p.split - 1) / p.split;
+    while (p.split > 1 && (p.split - 1) * p.part >= g.steps) p.split /= 2, p.part = (g.steps + p.split - 1) / p.split;
+    g.tmem_cols = 32;
+    while (g.tmem_cols < g.bn) g.tmem_cols *= 2;
+    Scratch sums(p.split > 1 ? static_cast<std::size_t>(ntiles) * p.split * g.bn * kTileM * sizeof(int) : 16);
+    p.sums = sums.as<int>();
+    g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (kTileM >> 4) << 24;
+    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn);
+    constexpr unsigned kMaxSmem = 222 * 1024;
+    static bool configured = false;
+    if (!configured) {
+        VC_CUDA(cudaFuncSetAttribute(matmul_q8_split, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
+        configured = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ntiles * p.split);
+    cfg.blockDim = dim3(kTcThreads);
+    cfg.dynamicSmemBytes = g.stages * stage + 1024;
+    cfg.stream = stream();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = p.split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    VC_CUDA(cudaLaunchKernelEx(&cfg, matmul_q8_split, bmap, amap, p));
+    check_launch("matmul_q8_split");
+}
+
 void check_q8_in(const char* name, const void* p, std::size_t pitch, std::size_t k) {
     if (pitch < k || pitch % 16 != 0 || !aligned16(p))
         fail(VC_ERR_INVALID, std::string("matmul_q8: the rows of ") + name +
@@ -651,8 +839,10 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
     if (k == 0) {
         matmul_q8_empty<<<grid_for(m * n, 256), 256, 0, stream()>>>(a_scale, b_scale, bias, g.m, g.n, out);
         check_launch("matmul_q8_empty");
-    } else if (m <= 32) {
+    } else if (m <= kRowsTokens) {
         launch_rows(g);
+    } else if (2 * ((n + kTileM - 1) / kTileM) * ((m + 255) / 256) <= static_cast<size_t>(sm_count())) {
+        launch_split(g);
     } else {
         launch_tc(g, m > 128);
     }
