@@ -464,7 +464,7 @@ vc_status vc_cuda_rms_norm(const float* x, size_t x_stride, const float* residua
  * be NULL: zero): with t = gy * weight,
  * dh = rstd * (t - h * (rstd^2 * mean(t * h))) + gh -- the gradient of x and of
  * residual alike -- and dw[j] = sum over rows of gy * (h * rstd). dh or dw may
- * be NULL to skip. All tensors contiguous; dh may be gy or gh itself. */
+ * be NULL to skip. All tensors contiguous; dh may be h, gy or gh itself. */
 vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const float* rstd, const float* gy,
                                     const float* gh, size_t rows, size_t cols, float* dh, float* dw);
 

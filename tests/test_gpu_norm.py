@@ -139,6 +139,35 @@ def test_odd_rows(backend, cols):
     within(y[[0, 5, 6]], want, R.rms_norm_bound(want), "rows beside odd ones")
 
 
+@pytest.mark.parametrize("rows,cols", [(50, 1030), (50, 4096), (3000, 1024), (1000, 4096), (700, 8192), (3, 40000)])
+@pytest.mark.parametrize("over", ["gy", "gh", "h"])
+def test_gradient_in_place(backend, rows, cols, over):
+    """dh written over one of the tensors it is computed from, which dw reads too."""
+    rng, x, _, w = inputs(rows, cols, 2)
+    gy, gh = (rng.normal(size=(rows, cols)).astype(np.float32) for _ in range(2))
+    d = {"h": backend.upload(x), "gy": backend.upload(gy), "gh": backend.upload(gh)}
+    dw_ = backend.upload(w)
+    _, _, rstd = backend.rms_norm(d["h"], dw_, rows, cols)
+    dw = backend.allocate(cols)
+    backend.rms_norm_backward(d["h"], dw_, rstd, d["gy"], rows, cols, gh=d["gh"], out=(d[over], dw))
+    edh, edw, bdh, bdw = R.rms_norm_backward(x, w, 1e-6, gy, gh)
+    within(backend.download(d[over]).reshape(rows, cols), edh, bdh, "dh")
+    within(backend.download(dw), edw, bdw, "dw")
+
+
+@pytest.mark.parametrize("rows,cols", [(160000, 64), (2049, 33), (5000, 1030), (90000, 128)])
+def test_long_sums_over_rows(backend, rows, cols):
+    """dw over more rows than one run of float additions takes."""
+    rng, x, _, w = inputs(rows, cols, 3)
+    gy = rng.normal(size=(rows, cols)).astype(np.float32)
+    dx, dw_ = backend.upload(x), backend.upload(w)
+    _, _, rstd = backend.rms_norm(dx, dw_, rows, cols)
+    dh, dw = backend.rms_norm_backward(dx, dw_, rstd, backend.upload(gy), rows, cols)
+    edh, edw, bdh, bdw = R.rms_norm_backward(x, w, 1e-6, gy, None)
+    within(backend.download(dh).reshape(rows, cols), edh, bdh, "dh")
+    within(backend.download(dw), edw, bdw, "dw")
+
+
 def test_no_rows_and_repeatable(backend):
     w = backend.upload(np.ones(40, np.float32))
     empty = backend.allocate(0)

@@ -379,21 +379,33 @@ struct NormBwdArgs {
     float* dh;
 };
 
-// dh, one row a CTA (or a warp) as in the forward: h and t = gy * w stay in
-// registers.
+// dh and dw in one launch, for what the ring below does not take: few rows, odd
+// lengths. The first CTAs write dh: groups of T threads, 1024 / T of them a CTA,
+// have a row each, h and t = gy * w in registers. The others add up dw: 32
+// columns a CTA, a slice of at most kDwRows of its rows a warp in float, the
+// slices in double and in order. Rows beyond 32 slices go to further CTAs whose
+// sums norm_dw_finish adds.
+constexpr unsigned kDwRows = 64;          // float additions in a row of a sum
+constexpr unsigned kDwSpan = 32 * kDwRows;  // rows a CTA adds up
+
+struct BothArgs {
+    NormBwdArgs n;
+    unsigned T, dh_ctas, column_ctas;
+    float* dw;  // or partial rows, one for each kDwSpan rows
+};
+
 template <bool SKEWED, int NV>
-__global__ void __launch_bounds__(1024)
-norm_bwd_dh(const NormBwdArgs a) {
-    __shared__ double ssum[32];
-    __shared__ float unused[32];
-    const unsigned long long row = static_cast<unsigned long long>(blockIdx.x) * blockDim.y + threadIdx.y;
-    if (row >= a.rows) return;
-    const unsigned T = blockDim.x, t = threadIdx.x;
+__device__ __forceinline__ void dh_of_rows(const BothArgs& b, double* slots) {
+    const NormBwdArgs& a = b.n;
+    const unsigned T = b.T, R = 1024 / T, group = threadIdx.x / T, t = threadIdx.x - group * T;
+    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned long long row = static_cast<unsigned long long>(blockIdx.x) * R + group;
+    if (row >= a.rows) return;  // a whole group
     const float* hp = a.h + row * a.cols;
     const float* gp = a.gy + row * a.cols;
     const Span span{SKEWED ? skew_of(hp) : 0, a.cols};
     const unsigned G = span.groups();
-    const float s = a.rstd[row];
+    const float s = __ldg(a.rstd + row);
     Group h[NV], g[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -416,7 +428,12 @@ norm_bwd_dh(const NormBwdArgs a) {
             dot += part;
         }
     }
-    dot = reduce_row<NORM_F32>(dot, 0.0f, ssum, unused).sq;
+    dot = warp_sum(dot);
+    if (T > 32) {  // the group's warps, in order
+        if (lane == 0) slots[warp] = dot;
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(T) : "memory");
+        dot = warp_sum(lane < T >> 5 ? slots[group * (T >> 5) + lane] : 0.0);
+    }
     const float c = static_cast<float>(dot / a.cols) * (s * s);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -424,16 +441,45 @@ norm_bwd_dh(const NormBwdArgs a) {
         if (at < G) {
             const Group up = a.gh ? load_group<SKEWED>(a.gh + row * a.cols, at, span) : Group{};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float v = s * (g[i].v[e] - h[i].v[e] * c);
-                g[i].v[e] = a.gh ? v + up.v[e] : v;
-            }
+            for (int e = 0; e < 4; ++e) g[i].v[e] = fmaf(s, fmaf(-h[i].v[e], c, g[i].v[e]), up.v[e]);
             store_group<SKEWED>(a.dh + row * a.cols, at, g[i], span);
         }
     }
 }
 
-// The same for rows too long for registers, or tensors of unlike alignment.
+__device__ __forceinline__ void dw_of_columns(const BothArgs& b, double (*part)[33]) {
+    const NormBwdArgs& a = b.n;
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned at = blockIdx.x - b.dh_ctas, segment = at / b.column_ctas, j = (at - segment * b.column_ctas) * 32 + lane;
+    const unsigned long long base = static_cast<unsigned long long>(segment) * kDwSpan;
+    const unsigned rows = static_cast<unsigned>(min(static_cast<unsigned long long>(kDwSpan), a.rows - base));
+    const unsigned per = (rows + 31) / 32, first = min(rows, warp * per), last = min(rows, first + per);
+    float sum = 0.0f;
+    if (j < a.cols) {
+        const float* gy = a.gy + (base + first) * a.cols + j;
+        const float* h = a.h + (base + first) * a.cols + j;
+#pragma unroll 8
+        for (unsigned i = first; i < last; ++i, gy += a.cols, h += a.cols)
+            sum = fmaf(*gy, *h * __ldg(a.rstd + base + i), sum);
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && j < a.cols) {
+        double all = 0.0;
+        for (unsigned v = 0; v < 32; ++v) all += part[v][lane];
+        b.dw[static_cast<unsigned long long>(segment) * a.cols + j] = static_cast<float>(all);
+    }
+}
+
+template <bool SKEWED, int NV>
+__global__ void __launch_bounds__(1024)
+norm_bwd_both(const BothArgs b) {
+    __shared__ double part[32][33];
+    if (blockIdx.x < b.dh_ctas) dh_of_rows<SKEWED, NV>(b, part[0]);
+    else dw_of_columns(b, part);
+}
+
+// dh for rows too long for registers, or tensors of unlike alignment.
 __global__ void __launch_bounds__(1024)
 norm_bwd_dh_long(const NormBwdArgs a) {
     __shared__ double scratch[32];
@@ -477,26 +523,6 @@ norm_dw_finish(const float* __restrict__ partial, unsigned long long count, unsi
 void launch_dw_finish(const float* partial, unsigned long long count, unsigned cols, float* dw) {
     launch_pdl(norm_dw_finish, dim3((cols + 31) / 32), dim3(1024), 0, stream(), partial, count, cols, dw);
     check_launch("norm_dw_finish");
-}
-
-// dw over segments of kDwRows rows, a column a thread, added in float; the
-// segments are then added in double.
-constexpr unsigned kDwRows = 64;
-
-__global__ void __launch_bounds__(128)
-norm_bwd_dw(const NormBwdArgs a, float* __restrict__ partial) {
-    const unsigned j = blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= a.cols) return;
-    const unsigned long long first = static_cast<unsigned long long>(blockIdx.y) * kDwRows;
-    const unsigned rows = static_cast<unsigned>(min(static_cast<unsigned long long>(kDwRows), a.rows - first));
-    const float* gy = a.gy + first * a.cols + j;
-    const float* h = a.h + first * a.cols + j;
-    float sum = 0.0f;
-#pragma unroll 8
-    for (unsigned i = 0; i < rows; ++i)
-        sum += gy[static_cast<unsigned long long>(i) * a.cols] *
-               (h[static_cast<unsigned long long>(i) * a.cols] * __ldg(a.rstd + first + i));
-    partial[static_cast<unsigned long long>(blockIdx.y) * a.cols + j] = sum;
 }
 
 // dh and dw from one pass over h, gy and gh, for aligned rows of up to
@@ -729,25 +755,31 @@ bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
     return true;
 }
 
-template <bool SKEWED>
-void launch_dh(const NormBwdArgs& a) {
-    const RowShape s = row_shape(a.cols, SKEWED, a.rows);
-    const unsigned long long ctas = (a.rows + s.rows - 1) / s.rows;
-    const dim3 block(s.threads, s.rows);
-    const unsigned grid = static_cast<unsigned>(ctas);
-    if (s.per <= 1) norm_bwd_dh<SKEWED, 1><<<grid, block, 0, stream()>>>(a);
-    else norm_bwd_dh<SKEWED, 4><<<grid, block, 0, stream()>>>(a);
-    check_launch("norm_bwd_dh");
-}
-
-void launch_dw(const NormBwdArgs& a, float* dw) {
-    const unsigned long long segments = (a.rows + kDwRows - 1) / kDwRows;
-    if (segments > 65535) fail(VC_ERR_OVERFLOW, "rms_norm_backward: too many rows");
-    Scratch partial(segments * a.cols * sizeof(float));
-    norm_bwd_dw<<<dim3((a.cols + 127) / 128, static_cast<unsigned>(segments)), 128, 0, stream()>>>(
-        a, segments > 1 ? partial.as<float>() : dw);
-    check_launch("norm_bwd_dw");
-    if (segments > 1) launch_dw_finish(partial.as<float>(), segments, a.cols, dw);
+void launch_both(const NormBwdArgs& n, float* dw, bool skewed) {
+    BothArgs b{};
+    b.n = n;
+    const unsigned groups = skewed ? (n.cols + 3 + 3) / 4 : n.cols / 4;
+    // as many threads a row as there are groups while rows are few, else a
+    // quarter; 64 would need a sixteenth named barrier
+    const unsigned want = n.rows * groups <= 1024ull * static_cast<unsigned>(sm_count()) ? 1 : 4;
+    b.T = 32;
+    while (b.T < 1024 && b.T * want < groups) b.T *= b.T == 32 ? 4 : 2;
+    const unsigned R = 1024 / b.T, per = (groups + b.T - 1) / b.T;
+    const unsigned long long dh_ctas = n.dh ? (n.rows + R - 1) / R : 0;
+    const unsigned long long segments = dw ? (n.rows + kDwSpan - 1) / kDwSpan : 0;
+    b.column_ctas = (n.cols + 31) / 32;
+    const unsigned long long ctas = dh_ctas + segments * b.column_ctas;
+    if (ctas > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm_backward: tensor too large");
+    b.dh_ctas = static_cast<unsigned>(dh_ctas);
+    Scratch partial(segments > 1 ? segments * n.cols * sizeof(float) : 16);
+    b.dw = segments > 1 ? partial.as<float>() : dw;
+    const auto launch = [&](auto kernel) { kernel<<<static_cast<unsigned>(ctas), 1024, 0, stream()>>>(b); };
+    if (skewed && per <= 1) launch(norm_bwd_both<true, 1>);
+    else if (skewed) launch(norm_bwd_both<true, 4>);
+    else if (per <= 1) launch(norm_bwd_both<false, 1>);
+    else launch(norm_bwd_both<false, 4>);
+    check_launch("norm_bwd_both");
+    if (segments > 1) launch_dw_finish(b.dw, segments, n.cols, dw);
 }
 
 void check_rows_cols(const char* what, std::size_t rows, std::size_t cols) {
@@ -839,19 +871,22 @@ vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const f
     if (rows > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm_backward: too many rows");
     NormBwdArgs a{h, weight, rstd, gy, gh, rows, static_cast<unsigned>(cols), dh};
     if (dh && dw && try_bwd_ring(a, dw)) return VC_OK;
-    if (dw) launch_dw(a, dw);
-    if (dh) {
-        const bool alike = same_skew(h, cols, gy, cols, rows) && same_skew(h, cols, gh, cols, rows) &&
-                           same_skew(h, cols, dh, cols, rows);
-        const bool skewed = cols % 4 != 0 || !aligned16(h) || !aligned16(weight);
-        if (!fits(a.cols, kNormBwdRegCols, skewed) || !alike) {
-            norm_bwd_dh_long<<<static_cast<unsigned>(rows), 1024, 0, stream()>>>(a);
-            check_launch("norm_bwd_dh_long");
-        } else if (skewed) {
-            launch_dh<true>(a);
-        } else {
-            launch_dh<false>(a);
-        }
+    const bool alike = same_skew(h, cols, gy, cols, rows) && same_skew(h, cols, gh, cols, rows) &&
+                       same_skew(h, cols, dh, cols, rows);
+    const bool skewed = cols % 4 != 0 || !aligned16(h) || !aligned16(weight);
+    // dw reads what dh may be written over: then it goes first, in a launch of its own
+    const bool over = dh == gy || dh == h, by_itself = dh && (!alike || !fits(a.cols, kNormBwdRegCols, skewed));
+    if (dw && dh && (over || by_itself)) {
+        a.dh = nullptr;
+        launch_both(a, dw, skewed);
+        a.dh = dh;
+        dw = nullptr;
+    }
+    if (by_itself) {
+        norm_bwd_dh_long<<<static_cast<unsigned>(rows), 1024, 0, stream()>>>(a);
+        check_launch("norm_bwd_dh_long");
+    } else {
+        launch_both(a, dw, skewed);
     }
     VC_API_END
 }
