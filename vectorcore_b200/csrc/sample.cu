@@ -21,10 +21,10 @@
 // is run again among the classes ahead of it. Sums are added in a fixed order
 // (four weights in float, then in double), so nothing depends on scheduling.
 //
-// A small k has its classes listed and sorted: they lie in the bins (of (m - l)
-// / T, 64 a unit) down to the k-th largest of the threads' own maxima. A large
-// k, or more equal logits than the list holds, has its last class found by five
-// histograms of the order's key, (ordered logit bits, ~index), 11 bits each.
+// A small k has its classes listed and sorted: none of them is below the k-th
+// largest of the maxima of some 2k groups of threads. A large k, or more equal
+// logits than the list holds, has its last class found by five histograms of the
+// order's key, (ordered logit bits, ~index), 11 bits each.
 //
 // Without top-k and min-p a row is read once from HBM, the sum and the race
 // running against the maximum so far; with them, once for its maximum. What
@@ -34,7 +34,7 @@
 // subtraction, one division, expf. `quick` is one product and ex2.approx,
 // within 2^-15 of it: it serves the sums, and decides whatever it can decide; a
 // race within 2^-14, or a class that near min_p, is decided by `weight`. A warp
-// looks at scores one by one only where one of its classes comes near the
+// passes over 128 classes at once where none of them is left, or comes near the
 // warp's leader.
 #include "vc_internal.cuh"
 
@@ -51,6 +51,7 @@ using u64 = unsigned long long;
 
 constexpr unsigned kBins = 2048;       // of a histogram
 constexpr unsigned kSorted = 512;      // classes a sorted list holds, over the cluster
+constexpr unsigned kGroups = 512;      // of threads, over the cluster, whose maxima bound the top k
 constexpr unsigned kMaxWarps = 32;
 constexpr unsigned kIndexBits = 23;    // a key is 32 ordered logit bits, then these of ~index
 constexpr std::size_t kMaxVocab = 1u << kIndexBits;
@@ -130,12 +131,6 @@ struct Weigh {
     __device__ __forceinline__ float4 quick(const float4& v) const {
         return make_float4(quick(v.x), quick(v.y), quick(v.z), quick(v.w));
     }
-    // larger logits never have a larger bin; masked classes have the last
-    __device__ __forceinline__ unsigned bin(float x) const {
-        const float to_bin = fminf(to_log2 * 44.0f, 1e30f);  // finite: 0 * to_bin is 0
-        const float b = fminf((m - capped(x)) * to_bin, static_cast<float>(kBins - 1)) + 8388608.0f;
-        return __float_as_uint(b) & 0x7fffffu;
-    }
     // w >= least, w being the quick weight of x
     __device__ __forceinline__ bool reaches(float least, float w, float x) const {
         if (w >= least * (1.0f + kNear)) return true;
@@ -147,6 +142,8 @@ struct Weigh {
 struct Shared {
     unsigned count[kBins];
     u64 pick[kSorted], sorted[kSorted];
+    float4 group[kGroups / 4];  // maxima of groups of threads, over the cluster
+    float cut;
     u64 warp64[kMaxWarps];
     double warpd[kMaxWarps];
     unsigned picked;
@@ -297,23 +294,6 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
     __syncthreads();
 }
 
-// The least float whose bin is at most b (a warp looks at 32 places at a time):
-// comparing with it stands for comparing bins.
-__device__ __forceinline__ float bin_end(const Weigh& wt, unsigned b) {
-    const unsigned lane = threadIdx.x & 31;
-    unsigned low = ordered(-kLargest), high = ordered(wt.m);  // the bin of high is 0
-    while (low < high) {
-        const unsigned step = (high - low) / 32 + 1;
-        const unsigned at = min(low + lane * step, high);
-        const unsigned reach = __ballot_sync(0xffffffffu, wt.bin(from_ordered(at)) <= b);
-        const unsigned first = reach ? __ffs(reach) - 1 : 32;  // bins fall along the lanes
-        if (first == 0) return from_ordered(low);
-        high = min(first < 32 ? low + first * step : high, high);
-        low = min(low + (first - 1) * step, high) + 1;
-    }
-    return from_ordered(high);
-}
-
 // The definition's score of a class, as a key: the lower index of equal ones.
 __device__ __noinline__ u64 exact_score(float x, float e, unsigned i, float m, float t) {
     Weigh wt;
@@ -338,15 +318,26 @@ struct Race {
     __device__ __forceinline__ void one(const Weigh& wt, float score, unsigned i) {
         if (!(score >= bound)) return;
         bool ahead = score > lead;
-        if (leader != 0xffffffffu && !(fabsf(score - lead) >= lead * kNear)) ahead = exact(wt, i) > exact(wt, leader);
+        if (leader != 0xffffffffu && leader != i && !(fabsf(score - lead) >= lead * kNear))
+            ahead = exact(wt, i) > exact(wt, leader);
         if (ahead) lead = score, leader = i;
     }
     // a quad's, all lanes of a warp together
     __device__ __forceinline__ void run(const Weigh& wt, const float4& w, const float4& e, unsigned i) {
         const float4 score = make_float4(quotient_quick(w.x, e.x), quotient_quick(w.y, e.y), quotient_quick(w.z, e.z),
                                          quotient_quick(w.w, e.w));
-        if (!__any_sync(0xffffffffu, largest(score) >= bound)) return;
-        one(wt, score.x, i), one(wt, score.y, i + 1), one(wt, score.z, i + 2), one(wt, score.w, i + 3);
+        const float high = largest(score);
+        if (!__any_sync(0xffffffffu, high >= bound)) return;
+        if (high >= bound) {
+            const float near = high * (1.0f - kNear);
+            const bool x1 = score.x >= near, y1 = score.y >= near, z1 = score.z >= near, w1 = score.w >= near;
+            one(wt, high, x1 ? i : y1 ? i + 1 : z1 ? i + 2 : i + 3);
+            if (x1 + y1 + z1 + w1 > 1) {  // the others that are as good
+                if (y1) one(wt, score.y, i + 1);
+                if (z1) one(wt, score.z, i + 2);
+                if (w1) one(wt, score.w, i + 3);
+            }
+        }
         float most = lead;
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
@@ -523,15 +514,18 @@ sample_kernel(const SampleArgs a) {
             constexpr int quads = decltype(loose)::value ? 1 : 2;
             const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
             float4 w[quads], e[quads];
+            bool any[quads];
 #pragma unroll
             for (int j = 0; j < quads; ++j) {
                 const unsigned i = first + j * 4 * THREADS;
                 w[j] = wt.quick(v[j]);
                 joins(v[j], i, w[j]);
-                e[j] = race.numbers(w[j], i, even);
+                any[j] = __any_sync(0xffffffffu, largest(w[j]) > 0.0f);
+                if (any[j]) e[j] = race.numbers(w[j], i, even);
             }
 #pragma unroll
-            for (int j = 0; j < quads; ++j) race.run(wt, w[j], e[j], first + j * 4 * THREADS);
+            for (int j = 0; j < quads; ++j)
+                if (any[j]) race.run(wt, w[j], e[j], first + j * 4 * THREADS);
         });
     };
 
@@ -579,11 +573,23 @@ sample_kernel(const SampleArgs a) {
     u64 top = block_max64(peak.at != 0xffffffffu ? key_of(x[peak.at], peak.at) : 0, s);
     if (t == 0) s.picked = 0;
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
-    if (C > 1) {
-        tell_all(cluster, s, [&](Shared& o) { o.top[rank] = top; });
-        cluster.sync();
-        for (unsigned r = 0; r < C; ++r) top = max(top, s.top[r]);
+    // the maxima of groups of neighbouring threads, 2k groups if there are as many
+    const bool few = k && k <= kSorted / 2;
+    const unsigned warps = C * THREADS / 32;  // of the cluster, at most 256
+    unsigned per_warp = 1;                    // groups
+    if (few) {
+        while (per_warp < 32 && 2 * per_warp * warps <= kGroups && per_warp * warps < 2 * k) per_warp *= 2;
+        float high = own_peak;
+        for (unsigned m = 1; m < 32 / per_warp; m <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, m));
+        const unsigned lanes = 32 / per_warp, lane = t & 31;
+        if (lane % lanes == 0)
+            for (unsigned r = 0; r < C; ++r)
+                reinterpret_cast<float*>(cluster.map_shared_rank(&s, r)->group)[(rank * THREADS / 32 + (t >> 5)) * per_warp +
+                                                                              lane / lanes] = high;
     }
+    tell_all(cluster, s, [&](Shared& o) { o.top[rank] = top; });
+    row_sync(cluster);
+    for (unsigned r = 0; r < C; ++r) top = max(top, s.top[r]);
     if (top == 0) {  // nothing in play, in any CTA of the cluster
         if (rank == 0 && t == 0) {
             a.token[row] = -1;
@@ -595,17 +601,25 @@ sample_kernel(const SampleArgs a) {
     if (at_once) total *= peak.at != 0xffffffffu ? exp2_quick((wt.m - high) * wt.to_log2) : 0.0f;
     wt.m = high;
 
-    // A small k: the bins of the threads' maxima down to the k-th hold the top k.
+    // A small k: the k-th largest of the groups' maxima is a lower bound of the top k.
     bool listing = false;
     float list_from = -INFINITY;
-    if (k && k <= kSorted / 2) {
-        clear_bins(s);
-        if (in_play(own_peak)) atomicAdd(&s.count[wt.bin(own_peak)], 1u);
-        const unsigned last_bin = find_bin(s, k).bin;
-        if (last_bin < kBins - 1) {  // the last bin has no lower end
-            listing = true;
-            list_from = bin_end(wt, last_bin);
+    const unsigned groups = warps * per_warp;
+    if (few && k <= groups) {
+        for (unsigned g = t; g < groups; g += THREADS) {
+            const float mine = reinterpret_cast<const float*>(s.group)[g];
+            unsigned place = 0;
+#pragma unroll 4
+            for (unsigned i = 0; i < groups; i += 4) {
+                const float4 o = s.group[i / 4];
+                place += (o.x > mine || (o.x == mine && i < g)) + (o.y > mine || (o.y == mine && i + 1 < g)) +
+                         (o.z > mine || (o.z == mine && i + 2 < g)) + (o.w > mine || (o.w == mine && i + 3 < g));
+            }
+            if (place == k - 1) s.cut = mine;
         }
+        __syncthreads();
+        list_from = s.cut;
+        listing = in_play(list_from);
     }
     // The row's sum, and with it the list, or the race of the classes that min-p
     // leaves.
@@ -699,7 +713,7 @@ sample_kernel(const SampleArgs a) {
         const Ahead ahead(key_of(x[i], i));
         double mass = 0.0;
         each_quad<4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
-            mass += sum4(ahead.only(v, j, wt.quick(v)));
+            if (__any_sync(0xffffffffu, largest(v) >= ahead.x)) mass += sum4(ahead.only(v, j, wt.quick(v)));
         });
         if (mass_of_all(mass, slot) < limit) break;
         race.restart();
