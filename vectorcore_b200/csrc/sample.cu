@@ -201,6 +201,19 @@ __device__ __forceinline__ Scan block_scan(u64 v, Shared& s) {
     return Scan{i - v + (warp ? ahead : 0), __shfl_sync(0xffffffffu, w, 31)};
 }
 
+__device__ __forceinline__ float block_max_f(float v, Shared& s) {
+    const unsigned lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    __syncthreads();
+    if (lane == 0) s.warp64[threadIdx.x >> 5] = __float_as_uint(v);
+    __syncthreads();
+    v = lane < warps ? __uint_as_float(static_cast<unsigned>(s.warp64[lane])) : -INFINITY;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+
 // A barrier of the row's CTAs.
 __device__ __forceinline__ void row_sync(const cg::cluster_group& cluster) {
     if (cluster.num_blocks() == 1) __syncthreads();
@@ -215,59 +228,102 @@ __device__ __forceinline__ void tell_all(const cg::cluster_group& cluster, Share
 
 // Classes are passed on by fours: v holds those at i .. i + 3, the ones outside
 // the range as masked (-inf), 16 bytes a load where the row allows it. A batch
-// is DEPTH quads, blockDim.x of them apart, loaded together:
+// is DEPTH quads, THREADS of them apart, loaded together:
 // f(quads, index of the first quad, loose). Whole warps come along, in the order
 // of the classes, but for the ends that are off the 16-byte grid: these come
 // last, one in the first place of a quad and `loose` true.
-template <int DEPTH, typename F>
+template <unsigned THREADS, int DEPTH, typename F>
 __device__ __forceinline__ void each_batch(const float* __restrict__ x, unsigned begin, unsigned end, F&& f) {
-    const unsigned t = threadIdx.x, threads = blockDim.x;
+    const unsigned t = threadIdx.x;
     const unsigned skew = static_cast<unsigned>((reinterpret_cast<std::uintptr_t>(x + begin) >> 2) & 3);
     const unsigned head = min(end, begin + ((4 - skew) & 3));
     const unsigned groups = (end - head) >> 2;
     const float4* body = reinterpret_cast<const float4*>(x + head);
     const float4 masked = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    for (unsigned g = t; (g & ~31u) < groups; g += DEPTH * threads) {
-        float4 v[DEPTH];
+    unsigned g = t;
+    if constexpr (DEPTH > 1)
+        for (; (g | 31u) + (DEPTH - 1) * THREADS < groups; g += DEPTH * THREADS) {
+            float4 v[DEPTH];
 #pragma unroll
-        for (int j = 0; j < DEPTH; ++j) v[j] = g + j * threads < groups ? body[g + j * threads] : masked;
+            for (int j = 0; j < DEPTH; ++j) v[j] = body[g + j * THREADS];
+            f(v, head + 4 * g, std::false_type{});
+        }
+    for (; (g & ~31u) < groups; g += THREADS) {
+        float4 v[1];
+        v[0] = g < groups ? body[g] : masked;
         f(v, head + 4 * g, std::false_type{});
     }
+    // the ends that are off the 16-byte grid, one class a thread
     const unsigned tail = head + 4 * groups, loose = (head - begin) + (end - tail);
     if (t < 32 && loose) {
         const unsigned i = t < head - begin ? begin + t : tail + t - (head - begin);
-        float4 v[DEPTH];
-#pragma unroll
-        for (int j = 0; j < DEPTH; ++j) v[j] = masked;
+        float4 v[1];
+        v[0] = masked;
         if (t < loose) v[0].x = x[i];
         f(v, i, std::true_type{});
     }
 }
 
-template <int DEPTH, typename F>
+// The first quad on the grid of each thread (masked where there is none), and
+// its place.
+struct First {
+    float4 v;
+    unsigned i;
+    bool there;
+};
+__device__ __forceinline__ First first_quad(const float* __restrict__ x, unsigned begin, unsigned end) {
+    const unsigned skew = static_cast<unsigned>((reinterpret_cast<std::uintptr_t>(x + begin) >> 2) & 3);
+    First f;
+    f.i = min(end, begin + ((4 - skew) & 3)) + 4 * threadIdx.x;
+    f.there = f.i + 3 < end;
+    f.v = f.there ? *reinterpret_cast<const float4*>(x + f.i)
+                  : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    return f;
+}
+
+template <unsigned THREADS, int DEPTH, typename F>
 __device__ __forceinline__ void each_quad(const float* x, unsigned begin, unsigned end, F&& f) {
-    each_batch<DEPTH>(x, begin, end, [&](const float4 (&v)[DEPTH], unsigned i, auto loose) {
+    each_batch<THREADS, DEPTH>(x, begin, end, [&](const auto& v, unsigned i, auto loose) {
+        constexpr int quads = sizeof(v) / sizeof(float4);
 #pragma unroll
-        for (int j = 0; j < (decltype(loose)::value ? 1 : DEPTH); ++j) f(v[j], i + j * 4 * blockDim.x, loose);
+        for (int j = 0; j < quads; ++j) f(v[j], i + j * 4 * THREADS, loose);
     });
 }
 
 __device__ __forceinline__ float largest(const float4& v) { return fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)); }
+template <int N>
+__device__ __forceinline__ float largest(const float4 (&v)[N]) {
+    float m = largest(v[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) m = fmaxf(m, largest(v[j]));
+    return m;
+}
+__device__ __forceinline__ float sum4(const float4& w) { return (w.x + w.y) + (w.z + w.w); }
+template <int N>
+__device__ __forceinline__ float sum_of(const float4 (&w)[N]) {
+    float s = sum4(w[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) s += sum4(w[j]);
+    return s;
+}
 
 // The largest logit a warp has seen, and the first class that has it. Like
 // fmaxf it passes over NaN; +inf counts as the largest float.
 struct Peak {
     float high{-INFINITY};
     unsigned at{0xffffffffu};
-    // v at i, all lanes of a warp together
-    template <typename L>
-    __device__ __forceinline__ void see(const float4& v, unsigned i, L) {
-        if constexpr (L::value) take_loose(v, i);
-        else if (grows(v)) take(v, i);
+    // a batch from i on, all lanes of a warp together
+    template <unsigned THREADS, int N, typename L>
+    __device__ __forceinline__ void see(const float4 (&v)[N], unsigned i, L) {
+        if constexpr (L::value) {
+            take_loose(v[0], i);
+        } else if (grows(largest(v))) {
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                if (grows(largest(v[j]))) take(v[j], i + j * 4 * THREADS);
+        }
     }
-    __device__ __forceinline__ bool grows(const float4& v) const {
-        return __any_sync(0xffffffffu, capped(largest(v)) > high);
-    }
+    __device__ __forceinline__ bool grows(float most) const { return __any_sync(0xffffffffu, capped(most) > high); }
     __device__ __forceinline__ void take(const float4& v, unsigned i) {
         float top = capped(largest(v));
 #pragma unroll
@@ -322,27 +378,38 @@ struct Race {
             ahead = exact(wt, i) > exact(wt, leader);
         if (ahead) lead = score, leader = i;
     }
-    // a quad's, all lanes of a warp together
-    __device__ __forceinline__ void run(const Weigh& wt, const float4& w, const float4& e, unsigned i) {
-        const float4 score = make_float4(quotient_quick(w.x, e.x), quotient_quick(w.y, e.y), quotient_quick(w.z, e.z),
-                                         quotient_quick(w.w, e.w));
-        const float high = largest(score);
-        if (!__any_sync(0xffffffffu, high >= bound)) return;
-        if (high >= bound) {
+    // a batch's weights and random numbers, all lanes of a warp together
+    template <unsigned THREADS, int N>
+    __device__ __forceinline__ void run(const Weigh& wt, const float4 (&w)[N], const float4 (&e)[N], unsigned first) {
+        float4 score[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) score[j] = scores(w[j], e[j]);
+        if (!__any_sync(0xffffffffu, largest(score) >= bound)) return;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float high = largest(score[j]);
+            if (!(high >= bound)) continue;
+            const unsigned i = first + j * 4 * THREADS;
             const float near = high * (1.0f - kNear);
-            const bool x1 = score.x >= near, y1 = score.y >= near, z1 = score.z >= near, w1 = score.w >= near;
+            const bool x1 = score[j].x >= near, y1 = score[j].y >= near, z1 = score[j].z >= near, w1 = score[j].w >= near;
             one(wt, high, x1 ? i : y1 ? i + 1 : z1 ? i + 2 : i + 3);
             if (x1 + y1 + z1 + w1 > 1) {  // the others that are as good
-                if (y1) one(wt, score.y, i + 1);
-                if (z1) one(wt, score.z, i + 2);
-                if (w1) one(wt, score.w, i + 3);
+                if (y1) one(wt, score[j].y, i + 1);
+                if (z1) one(wt, score[j].z, i + 2);
+                if (w1) one(wt, score[j].w, i + 3);
             }
         }
         float most = lead;
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, m));
-        bound = fmaxf(most * (1.0f - kNear), 0x1p-149f);
+        bound = fmaxf(most * (1.0f - kNear), bound);
     }
+    __device__ __forceinline__ float4 scores(const float4& w, const float4& e) const {
+        return make_float4(quotient_quick(w.x, e.x), quotient_quick(w.y, e.y), quotient_quick(w.z, e.z),
+                           quotient_quick(w.w, e.w));
+    }
+    // a score that some class of the race reaches
+    __device__ __forceinline__ void start_from(float score) { bound = fmaxf(score * (1.0f - kNear), 0x1p-149f); }
     // the maximum that the weights are relative to grew
     __device__ __forceinline__ void rescale(float less) {
         lead *= less;
@@ -374,16 +441,16 @@ struct Found {
 __device__ __noinline__ Found find_bin(Shared& s, u64 target) {
     const cg::cluster_group cluster = cg::this_cluster();
     const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
-    const unsigned share = kBins / C, per = share >= blockDim.x ? share / blockDim.x : 1;  // per <= 4
+    const unsigned share = kBins / C, per = share >= blockDim.x ? share / blockDim.x : 1;  // per <= 8
     const unsigned first = rank * share + threadIdx.x * per;
     const bool any = threadIdx.x * per < share;
     __syncthreads();
     if (threadIdx.x == 0) s.found_bin = kBins;
     row_sync(cluster);
-    unsigned n[4] = {};
+    unsigned n[8] = {};
     if (any) {
 #pragma unroll
-        for (unsigned j = 0; j < 4; ++j) {
+        for (unsigned j = 0; j < 8; ++j) {
             if (j >= per) break;
             unsigned c[kMaxCluster];  // in flight together
 #pragma unroll
@@ -393,7 +460,9 @@ __device__ __noinline__ Found find_bin(Shared& s, u64 target) {
             for (unsigned r = 0; r < kMaxCluster; ++r) n[j] += c[r];
         }
     }
-    const u64 mine = static_cast<u64>(n[0]) + n[1] + n[2] + n[3];
+    u64 mine = 0;
+#pragma unroll
+    for (unsigned j = 0; j < 8; ++j) mine += n[j];
     const Scan scan = block_scan(mine, s);
     u64 c = scan.before;
     if (C > 1) {
@@ -404,7 +473,7 @@ __device__ __noinline__ Found find_bin(Shared& s, u64 target) {
     if (any && c < target && c + mine >= target) {
         unsigned j = 0;
 #pragma unroll
-        for (unsigned i = 0; i < 3; ++i)
+        for (unsigned i = 0; i < 7; ++i)
             if (j == i && c + n[i] < target) c += n[i], ++j;
         for (unsigned r = 0; r < C; ++r) {
             Shared* o = cluster.map_shared_rank(&s, r);
@@ -441,12 +510,13 @@ __device__ __noinline__ void sort_picks(Shared& s, unsigned n) {
 }
 
 // The key of the k-th class in order (k at most the classes in play).
+template <unsigned THREADS>
 __device__ __noinline__ u64 kth_key(Shared& s, const float* x, unsigned begin, unsigned end, u64 k) {
     u64 prefix = 0;
     for (unsigned shift = kKeyBits; shift > 0;) {
         shift -= kLevelBits;
         clear_bins(s);
-        each_quad<1>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 1>(x, begin, end, [&](const float4& v, unsigned i, auto) {
             const auto tally = [&](float u, unsigned j) {
                 if (!in_play(u)) return;
                 const u64 key = key_of(u, j);
@@ -506,35 +576,50 @@ sample_kernel(const SampleArgs a) {
     Peak peak;
     double total = 0.0;
     float own_peak = -INFINITY;  // this thread's
-    const auto sum4 = [](const float4& w) { return (w.x + w.y) + (w.z + w.w); };
     // Races the classes of the row that `joins(quad, index, weights)` leaves a
     // weight: their random numbers are fetched together before any is looked at.
+    // The best of each thread's first classes is known beforehand, so that few of
+    // the rest have to be compared one by one.
     const auto race_those = [&](auto&& joins) {
-        each_batch<2>(x, begin, end, [&](const float4 (&v)[2], unsigned first, auto loose) {
-            constexpr int quads = decltype(loose)::value ? 1 : 2;
-            const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
+        {
+            const First f = first_quad(x, begin, end);
+            float4 w = wt.quick(f.v);
+            const double kept = total;
+            joins(f.v, f.i, w);
+            total = kept;  // the pass below adds these too
+            const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + f.i) & 15) == 0;
+            const float score = largest(w) > 0.0f ? largest(race.scores(w, race.numbers(w, f.i, even))) : 0.0f;
+            race.start_from(fmaxf(block_max_f(score, s), 0.0f));
+        }
+        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
+            constexpr int quads = sizeof(v) / sizeof(float4);
+            const bool even = !decltype(loose)::value && (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
             float4 w[quads], e[quads];
-            bool any[quads];
 #pragma unroll
             for (int j = 0; j < quads; ++j) {
-                const unsigned i = first + j * 4 * THREADS;
                 w[j] = wt.quick(v[j]);
-                joins(v[j], i, w[j]);
-                any[j] = __any_sync(0xffffffffu, largest(w[j]) > 0.0f);
-                if (any[j]) e[j] = race.numbers(w[j], i, even);
+                joins(v[j], first + j * 4 * THREADS, w[j]);
             }
+            if (!__any_sync(0xffffffffu, largest(w) > 0.0f)) return;
 #pragma unroll
-            for (int j = 0; j < quads; ++j)
-                if (any[j]) race.run(wt, w[j], e[j], first + j * 4 * THREADS);
+            for (int j = 0; j < quads; ++j) e[j] = race.numbers(w[j], first + j * 4 * THREADS, even);
+            race.template run<THREADS>(wt, w, e, first);
         });
     };
 
     if (at_once) {
         // one pass: the sum and the race relative to the warp's maximum so far
-        wt.m = -kLargest;  // no class in play is below it
-        each_batch<2>(x, begin, end, [&](const float4 (&v)[2], unsigned first, auto loose) {
-            constexpr int quads = decltype(loose)::value ? 1 : 2;
-            float4 e[quads];
+        const First f = first_quad(x, begin, end);
+        wt.m = fmaxf(capped(block_max_f(largest(f.v), s)), -kLargest);  // no class in play is below that
+        if (!first_only) {
+            const float4 w = wt.quick(f.v);
+            const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + f.i) & 15) == 0;
+            const float score = largest(w) > 0.0f ? largest(race.scores(w, race.numbers(w, f.i, even))) : 0.0f;
+            race.start_from(fmaxf(block_max_f(score, s), 0.0f));
+        }
+        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
+            constexpr int quads = sizeof(v) / sizeof(float4);
+            float4 w[quads], e[quads];
             const bool even = !decltype(loose)::value && (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < quads; ++j) {
@@ -543,34 +628,33 @@ sample_kernel(const SampleArgs a) {
                 if (first_only) continue;
                 if constexpr (decltype(loose)::value) {
                     if (i < end) e[j].x = race.noise[i];
-                } else if (i + 3 < end) {  // a quad of the row, not past its last
+                } else if (quads > 1 || i + 3 < end) {  // a quad of the row, not past its last
                     if (even) e[j] = *reinterpret_cast<const float4*>(race.noise + i);
                     else
                         e[j] = make_float4(race.noise[i], race.noise[i + 1], race.noise[i + 2], race.noise[i + 3]);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < quads; ++j) {
-                const unsigned i = first + j * 4 * THREADS;
-                peak.see(v[j], i, loose);
-                if (peak.high > wt.m) {  // the whole warp
-                    const float less = exp2_quick((wt.m - peak.high) * wt.to_log2);
-                    total *= less;
-                    race.rescale(less);
-                    wt.m = peak.high;
-                }
-                const float4 w = wt.quick(v[j]);
-                total += sum4(w);
-                if (!first_only) race.run(wt, w, e[j], i);
+            peak.template see<THREADS>(v, first, loose);
+            if (peak.high > wt.m) {  // the whole warp
+                const float less = exp2_quick((wt.m - peak.high) * wt.to_log2);
+                total *= less;
+                race.rescale(less);
+                wt.m = peak.high;
             }
+#pragma unroll
+            for (int j = 0; j < quads; ++j) w[j] = wt.quick(v[j]);
+            total += sum_of(w);
+            if (!first_only) race.template run<THREADS>(wt, w, e, first);
         });
     } else {
-        each_quad<4>(x, begin, end, [&](const float4& v, unsigned i, auto loose) {
+        each_batch<THREADS, 4>(x, begin, end, [&](const auto& v, unsigned i, auto loose) {
             own_peak = fmaxf(own_peak, largest(v));
-            peak.see(v, i, loose);
+            peak.template see<THREADS>(v, i, loose);
         });
     }
-    u64 top = block_max64(peak.at != 0xffffffffu ? key_of(x[peak.at], peak.at) : 0, s);
+    u64 top = 0;
+    if (peak.at != 0xffffffffu) top = key_of(peak.high < kLargest ? peak.high : x[peak.at], peak.at);
+    top = block_max64(top, s);
     if (t == 0) s.picked = 0;
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
     // the maxima of groups of neighbouring threads, 2k groups if there are as many
@@ -598,7 +682,7 @@ sample_kernel(const SampleArgs a) {
         return;
     }
     const float high = capped(key_logit(top));
-    if (at_once) total *= peak.at != 0xffffffffu ? exp2_quick((wt.m - high) * wt.to_log2) : 0.0f;
+    if (at_once) total *= exp2_quick((wt.m - high) * wt.to_log2);
     wt.m = high;
 
     // A small k: the k-th largest of the groups' maxima is a lower bound of the top k.
@@ -624,7 +708,7 @@ sample_kernel(const SampleArgs a) {
     // The row's sum, and with it the list, or the race of the classes that min-p
     // leaves.
     if (k) {
-        each_quad<2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
             total += sum4(wt.quick(v));
             if (!listing || !(largest(v) >= list_from)) return;
             const auto lists = [&](float u, unsigned j) {
@@ -662,6 +746,7 @@ sample_kernel(const SampleArgs a) {
     };
     unsigned turn = 0;  // of the slots that go round
     bool sorted = false;
+    u64 listed_best = 0;  // of the sorted classes
     double limit = 0.0;
     if (k) {
         row_sync(cluster);
@@ -670,26 +755,43 @@ sample_kernel(const SampleArgs a) {
         sorted = listing && n <= kSorted;
         if (sorted) {
             if (rank == 0) {
-                // the classes in order, one a thread: the filters, then the race of the ones left
-                static_assert(kSorted <= THREADS, "one class a thread");
+                // the classes in order, `per` a thread: the filters, then the race of the ones left
+                constexpr unsigned per = kSorted > THREADS ? kSorted / THREADS : 1;
                 sort_picks(s, n);
-                const u64 key = t < n && t < k ? s.sorted[t] : 0;
-                const float v = key_logit(key), w = key ? wt.quick(v) : 0.0f;
-                const float e = key ? race.noise[key_index(key)] : 1.0f;
-                const u64 mass = __float2ull_rn(w * 0x1p40f);  // whole numbers: exact sums in any order
-                const Scan scan = block_scan(mass, s);
-                const bool left = !by_p || static_cast<double>(scan.before) <
-                                               static_cast<double>(p_in) * static_cast<double>(scan.all);
-                if (key && left && wt.reaches(min_p, w, v)) race.one(wt, quotient_quick(w, e), key_index(key));
+                u64 key[per], mass[per], sum = 0;
+                float w[per], e[per];
+#pragma unroll
+                for (unsigned j = 0; j < per; ++j) {
+                    const unsigned at = t * per + j;
+                    key[j] = at < n && at < k ? s.sorted[at] : 0;
+                    w[j] = key[j] ? wt.quick(key_logit(key[j])) : 0.0f;
+                    e[j] = key[j] ? race.noise[key_index(key[j])] : 1.0f;
+                    mass[j] = __float2ull_rn(w[j] * 0x1p40f);  // whole numbers: exact sums in any order
+                    sum += mass[j];
+                }
+                const Scan scan = block_scan(sum, s);
+                u64 before = scan.before;
+                const double most = static_cast<double>(p_in) * static_cast<double>(scan.all);
+#pragma unroll
+                for (unsigned j = 0; j < per; ++j) {
+                    const float v = key_logit(key[j]);
+                    if (key[j] && (!by_p || static_cast<double>(before) < most) && wt.reaches(min_p, w[j], v))
+                        listed_best = max(listed_best, exact_score(v, e[j], key_index(key[j]), wt.m, wt.t));
+                    before += mass[j];
+                }
             }
         } else {
-            const u64 least = kth_key(s, x, begin, end, k);
+            const u64 least = kth_key<THREADS>(s, x, begin, end, k);
             double mass = 0.0;
+            each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+                const auto keep = [&](float u, unsigned j) {
+                    return in_play(u) && key_of(u, j) >= least ? wt.quick(u) : 0.0f;
+                };
+                mass += sum4(make_float4(keep(v.x, i), keep(v.y, i + 1), keep(v.z, i + 2), keep(v.w, i + 3)));
+            });
             race_those([&](const float4& v, unsigned i, float4& w) {
                 const auto keep = [&](float u, unsigned j, float& w) {
-                    if (!in_play(u) || key_of(u, j) < least) w = 0.0f;
-                    mass += w;
-                    if (!wt.reaches(min_p, w, u)) w = 0.0f;
+                    if (!in_play(u) || key_of(u, j) < least || !wt.reaches(min_p, w, u)) w = 0.0f;
                 };
                 keep(v.x, i, w.x), keep(v.y, i + 1, w.y), keep(v.z, i + 2, w.z), keep(v.w, i + 3, w.w);
             });
@@ -701,7 +803,7 @@ sample_kernel(const SampleArgs a) {
     // below the limit, the race again among the classes ahead of it.
     u64 won;
     for (bool first_turn = true;; first_turn = false) {
-        const u64 mine = block_max64(race.best(wt), s);
+        const u64 mine = block_max64(sorted ? listed_best : race.best(wt), s);
         const unsigned slot = turn++ & 1;
         tell_all(cluster, s, [&](Shared& o) { o.best[slot][rank] = mine; });
         row_sync(cluster);
@@ -712,7 +814,7 @@ sample_kernel(const SampleArgs a) {
         const unsigned i = ~static_cast<unsigned>(won);
         const Ahead ahead(key_of(x[i], i));
         double mass = 0.0;
-        each_quad<4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
+        each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
             if (__any_sync(0xffffffffu, largest(v) >= ahead.x)) mass += sum4(ahead.only(v, j, wt.quick(v)));
         });
         if (mass_of_all(mass, slot) < limit) break;
@@ -743,8 +845,13 @@ void launch_rows(const SampleArgs& a, unsigned rows, unsigned C) {
     check_launch("sample_kernel");
 }
 
+// Up to here four CTAs of 256 threads an SM are faster than two of 512: a row is
+// mostly barriers (512 rows of 4000 classes: 22 us against 28; 256 of 128000,
+// the other way, 131 against 140).
+constexpr bool vocab_fits_four(unsigned vocab) { return vocab <= 16384; }
+
 // Few rows are bound by the latency of their passes: as many CTAs of 1024
-// threads a row as leave each an SM of its own and 2048 classes. With more
+// threads a row as leave each an SM of its own and 6400 classes. With more
 // rows, two CTAs of 512 threads an SM, so that one's passes run through the
 // other's barriers, and as many of them a row (which is read more than once
 // where there are filters) as keep the rows that run together within 48 MB:
@@ -753,12 +860,13 @@ void launch_sample(SampleArgs& a, std::size_t rows) {
     const u64 sms = static_cast<unsigned>(sm_count());
     const bool filtered = a.top_k || a.top_p || a.min_p;
     unsigned C = 1;
-    while (C < kMaxCluster && ((2 * rows * C <= sms && a.vocab / (2 * C) >= 2048) ||
+    while (C < kMaxCluster && ((2 * rows * C <= sms && a.vocab / (2 * C) >= 6400) ||
                                (filtered && rows > sms && 2 * sms / C * a.vocab * sizeof(float) > 48ull << 20)))
         C *= 2;
     a.chunk = ((a.vocab + C - 1) / C + 3) / 4 * 4;
     if (rows * C > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "sample: too many rows");
     if (rows * C <= sms) launch_rows<1024>(a, static_cast<unsigned>(rows), C);
+    else if (vocab_fits_four(a.vocab)) launch_rows<256>(a, static_cast<unsigned>(rows), C);
     else launch_rows<512>(a, static_cast<unsigned>(rows), C);
 }
 
