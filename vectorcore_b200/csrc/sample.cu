@@ -850,24 +850,27 @@ void launch_rows(const SampleArgs& a, unsigned rows, unsigned C) {
 // the other way, 131 against 140).
 constexpr bool vocab_fits_four(unsigned vocab) { return vocab <= 16384; }
 
-// Few rows are bound by the latency of their passes: as many CTAs of 1024
-// threads a row as leave each an SM of its own and 6400 classes. With more
-// rows, two CTAs of 512 threads an SM, so that one's passes run through the
-// other's barriers, and as many of them a row (which is read more than once
-// where there are filters) as keep the rows that run together within 48 MB:
-// beyond that L2 loses a row between its passes.
+// Few rows are bound by the latency of their passes and barriers: as many CTAs a
+// row as leave each an SM of its own and 3200 classes, of 512 threads up to 16384
+// classes and of 1024 beyond (1 x 32000: 8.9 us with 512, 10.6 with 1024; 48 x
+// 50257 the other way, 29 and 27). With more rows, two CTAs of 512 threads an SM,
+// so that one's passes run through the other's barriers, and as many of them a
+// row (which is read more than once where there are filters) as keep the rows
+// that run together within 48 MB: beyond that L2 loses a row between its passes
+// (160 x 200000: 110 us, with half as many CTAs a row 126).
 void launch_sample(SampleArgs& a, std::size_t rows) {
     const u64 sms = static_cast<unsigned>(sm_count());
     const bool filtered = a.top_k || a.top_p || a.min_p;
     unsigned C = 1;
-    while (C < kMaxCluster && ((2 * rows * C <= sms && a.vocab / (2 * C) >= 6400) ||
+    while (C < kMaxCluster && ((2 * rows * C <= sms && a.vocab / (2 * C) >= 3200) ||
                                (filtered && rows > sms && 2 * sms / C * a.vocab * sizeof(float) > 48ull << 20)))
         C *= 2;
     a.chunk = ((a.vocab + C - 1) / C + 3) / 4 * 4;
     if (rows * C > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "sample: too many rows");
-    if (rows * C <= sms) launch_rows<1024>(a, static_cast<unsigned>(rows), C);
-    else if (vocab_fits_four(a.vocab)) launch_rows<256>(a, static_cast<unsigned>(rows), C);
-    else launch_rows<512>(a, static_cast<unsigned>(rows), C);
+    const unsigned n = static_cast<unsigned>(rows);
+    if (rows * C <= sms && a.chunk > 16384) launch_rows<1024>(a, n, C);
+    else if (rows * C <= sms || !vocab_fits_four(a.vocab)) launch_rows<512>(a, n, C);
+    else launch_rows<256>(a, n, C);
 }
 
 }  // namespace
