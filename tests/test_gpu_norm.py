@@ -187,6 +187,7 @@ def test_no_rows_and_repeatable(backend):
 
 def test_refusals(backend):
     x, w = backend.upload(np.ones(64, np.float32)), backend.upload(np.ones(16, np.float32))
+    y = backend.allocate(64)
     for eps in (-1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError, match="eps"):
             backend.rms_norm(x, w, 4, 16, eps=eps)
@@ -203,6 +204,12 @@ def test_refusals(backend):
                  (x.ptr, 16, 4, 16, q.ptr + 8, 16, s.ptr), (x.ptr, 16, 4, 16, None, 16, s.ptr)):
         with pytest.raises(ValueError, match="pitch|null"):
             _abi.call("vc_cuda_quantize_q8", *args)
+    for name in ("vc_cuda_rms_norm", "vc_cuda_rms_norm_q8"):  # rows of x that overlap rows of h unlike
+        tail = (y.ptr, None) if name == "vc_cuda_rms_norm" else (q.ptr, 16, s.ptr)
+        with pytest.raises(ValueError, match="contiguous"):
+            _abi.call(name, x.ptr, 12, None, 0, w.ptr, 4, 16, 1e-6, x.ptr, *tail)
+        with pytest.raises(ValueError, match="contiguous"):
+            _abi.call(name, y.ptr, 16, x.ptr, 12, w.ptr, 4, 16, 1e-6, x.ptr, *tail)
     with pytest.raises(OverflowError):
         _abi.call("vc_cuda_rms_norm", x.ptr, 16, None, 0, w.ptr, 1 << 62, 16, 1e-6, None, x.ptr, None)
     with pytest.raises(OverflowError):

@@ -30,8 +30,8 @@ struct MatmulQ8Args {
 // 128-byte pieces of k in turn, 16 bytes a thread and load, and multiply them by
 // m16n8k32 products. A product's four groups of k may be any four as long as both
 // sides agree, so a thread's 16 consecutive bytes serve as they are; no byte is
-// moved between threads. The warps' sums meet in shared memory.
-constexpr unsigned kRowsTokens = 16;
+// moved between threads. The warps' sums meet in shared memory. 1 x 32000 x 4096
+// takes 24 us, 5.5 TB/s (the tensor-core tiles below 30); 1 x 4096 x 4096 5.9.
 constexpr unsigned kRowsWarps = 8;
 constexpr unsigned kPiece = 128;  // bytes of k a warp takes at a time
 
@@ -134,15 +134,12 @@ void launch_rows(const MatmulQ8Args& g) {
 // The weights b are the instruction's M side and the tokens a its N side, so a
 // tile's accumulators lie in TMEM with one weight row a lane: a warp's store of
 // one register is 32 neighbouring outputs of one token, coalesced whatever n's
-// alignment, with no trip through shared memory.
-//
-// One CTA an SM walks the tiles: a warp fetches 128-byte slices of k of both
-// sides by TMA (128-byte swizzle, zeros past the ends, so k, m and n need no
-// alignment), one thread of another issues the products (32 bytes of k each),
-// and eight warps scale and store the previous tile out of the other half of
-// TMEM meanwhile.
+// alignment, with no trip through shared memory. A warp of a CTA fetches
+// 128-byte slices of k of both sides by TMA (128-byte swizzle, zeros past the
+// ends, so k, m and n need no alignment), one thread of another issues the
+// products (32 bytes of k each), and eight warps scale and store.
 
-constexpr unsigned kTileM = 128;   // weight rows a tile: TMEM's lanes
+constexpr unsigned kTileM = 128;   // weight rows a CTA's tile: TMEM's lanes
 constexpr unsigned kSliceK = 128;  // bytes of k a stage: one swizzled row
 constexpr unsigned kMmaK = 32;     // bytes of k an instruction
 constexpr unsigned kStoreWarps = 8;  // two for each quarter of TMEM's lanes
@@ -159,7 +156,7 @@ struct TcArgs {
     unsigned tiles_m;     // along the tokens
     unsigned tiles_n;     // along the weights
     unsigned stages;
-    unsigned tmem_cols;   // allocated: both halves
+    unsigned tmem_cols;   // allocated
     unsigned idesc;
     unsigned* err;
 };
@@ -278,6 +275,7 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
 #pragma unroll
             for (unsigned j = 0; j < 16; ++j) s[j] = c + j < rows ? __ldg(sa + c + j) : 0.0f;
         }
+        __syncwarp();
         tmem_load_wait();
 #pragma unroll
         for (unsigned j = 0; j < 16; ++j) s[j] = static_cast<float>(v[j]) * (s[j] * sb);
@@ -285,7 +283,6 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
 #pragma unroll
             for (unsigned j = 0; j < 16; ++j) s[j] += bias;
         }
-        __syncwarp();
         if (c + step < rows) tmem_load16(taddr + c + step, v);
         float* out = g.out + static_cast<unsigned long long>(row0 + c) * g.n + col;
         if (mine && c + 16 <= rows) {
@@ -299,112 +296,17 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
     }
 }
 
-__global__ void __launch_bounds__(kTcThreads, 1)
-matmul_q8_tc(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const TcArgs g) {
-    extern __shared__ unsigned char smem_raw[];
-    unsigned char* tiles = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
-    __shared__ unsigned long long full[8], empty[8], acc_full[2], acc_empty[2];
-    __shared__ unsigned tmem_base, dead_flag;
-    volatile unsigned* dead = &dead_flag;
-    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr unsigned a_at = kTileM * kSliceK;
-    const unsigned stage_bytes = a_at + g.bn * kSliceK;
-    const unsigned ntiles = g.tiles_m * g.tiles_n;
-    if (threadIdx.x == 0) {
-        dead_flag = 0;
-        for (unsigned s = 0; s < g.stages; ++s) {
-            mbar_init(full + s, 1);
-            mbar_init(empty + s, 1);
-        }
-        for (unsigned s = 0; s < 2; ++s) {
-            mbar_init(acc_full + s, 1);
-            mbar_init(acc_empty + s, kStoreWarps);
-        }
-        mbar_fence_init();
-    }
-    if (warp == kStoreWarps + 1)
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_base)),
-                     "r"(g.tmem_cols)
-                     : "memory");
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const unsigned tmem = tmem_base;
-
-    if (warp == kStoreWarps) {  // fetch
-        if (lane == 0) {
-            Place at;
-            unsigned issued = 0;
-            bool ok = true;
-            for (unsigned i = blockIdx.x; ok && i < ntiles; i += gridDim.x) {
-                unsigned tn, tm;
-                tile_at(i, g, tn, tm);
-                for (unsigned s = 0; s < g.steps; ++s, ++issued, at.next(g.stages)) {
-                    unsigned long long* bar = full + at.slot;
-                    if (issued >= g.stages && !(ok = tc_wait<false>(empty + at.slot, at.parity ^ 1, dead, g.err))) break;
-                    unsigned char* dst = tiles + at.slot * stage_bytes;
-                    mbar_expect_tx(bar, stage_bytes);
-                    const int x = static_cast<int>(s * kSliceK);
-                    tma_load_2d(dst, &bmap, bar, x, static_cast<int>(tn * kTileM));
-                    tma_load_2d(dst + a_at, &amap, bar, x, static_cast<int>(tm * g.bn));
-                }
-            }
-            drain(full, issued, g);
-        }
-    } else if (warp == kStoreWarps + 1) {  // products
-        if (lane == 0) {
-            Place at;
-            unsigned turn = 0;
-            bool ok = true;
-            const unsigned long long da0 = tile_desc(smem_addr(tiles)), db0 = da0 + (a_at >> 4);
-            for (unsigned i = blockIdx.x; ok && i < ntiles; i += gridDim.x, ++turn) {
-                const unsigned half = turn & 1, d = tmem + half * g.bn;
-                if (turn > 1 && !(ok = tc_wait<false>(acc_empty + half, ((turn >> 1) - 1) & 1, dead, g.err))) break;
-                tc_fence_after();
-                for (unsigned s = 0; s < g.steps; ++s, at.next(g.stages)) {
-                    if (!(ok = tc_wait<false>(full + at.slot, at.parity, dead, g.err))) break;
-                    const unsigned long long skip = at.slot * (stage_bytes >> 4);
-#pragma unroll
-                    for (unsigned j = 0; j < kSliceK / kMmaK; ++j)
-                        mma_i8(d, da0 + skip + j * (kMmaK >> 4), db0 + skip + j * (kMmaK >> 4), g.idesc, s + j != 0);
-                    mma_commit(empty + at.slot);
-                }
-                if (ok) mma_commit(acc_full + half);
-            }
-        }
-    } else {  // scale and store
-        unsigned turn = 0;
-        for (unsigned i = blockIdx.x; i < ntiles; i += gridDim.x, ++turn) {
-            const unsigned half = turn & 1;
-            if (!tc_wait(acc_full + half, (turn >> 1) & 1, dead, g.err)) break;
-            tc_fence_after();
-            unsigned tn, tm;
-            tile_at(i, g, tn, tm);
-            store_tile(g, tmem + half * g.bn, tn * kTileM + (warp & 3) * 32, tm * g.bn);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty + half);
-        }
-    }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    if (warp == kStoreWarps + 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols));
-    }
-}
-
 // Too few tiles for the SMs: a cluster of S CTAs shares a tile, each taking its
 // part of k. A CTA hands every other one the sums of a share of the tokens and
 // adds up its own share, which it scales and stores. The sums meet in scratch
 // memory, which stays in L2: the cluster's shared memory takes some 15 bytes a
 // clock from its neighbours, L2 four times that (256 x 4096 x 4096 spent 12 of 21
-// us on the exchange by way of shared memory). One tile a CTA, no double buffer.
+// us on the exchange by way of shared memory, 16 in all without it). Clusters of
+// eight found fewer places on the GPU: 64 x 2048 x 4096 took 18 us with them, 10
+// with four. One tile a CTA, no double buffer.
 struct SplitArgs {
     TcArgs g;
-    unsigned split;       // CTAs a tile, a power of two up to 8
+    unsigned split;       // CTAs a tile, 1, 2 or 4
     unsigned part;        // steps along k a CTA
     int* sums;            // scratch: [tile][CTA of the cluster][token][weight row]
 };
@@ -546,12 +448,15 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
     }
 }
 
-// The same with pairs of CTAs on one tile of 256 weight rows: each CTA fetches
-// its own 128 weight rows and half of the tokens, and the instruction, issued by
-// the first CTA of the pair, reads both CTAs' shared memory: a third less to
-// fetch and to hold for a stage. A stage holds 256 bytes of k, eight products:
-// with 128 the one thread's wait, issue and commit took longer than the four
-// products they bring (8192^3: 385 us, with 256 324 us).
+// Tiles enough for all SMs: pairs of CTAs walk tiles of 256 weight rows by up to
+// 256 tokens. Each CTA fetches its own 128 weight rows and half of the tokens, and
+// the instruction, issued by the first CTA of the pair, reads both CTAs' shared
+// memory: a third less to fetch and to hold for a stage than one CTA's 128 x 256
+// tile. The previous tile leaves the other half of TMEM meanwhile. A stage holds
+// 256 bytes of k, eight products: with 128 the one thread's wait, issue and commit
+// took longer than the four products they bring (8192^3: 385 us with one CTA a
+// tile and 128 bytes, 313 this way: 3.5 Pop/s, twice the rate of a 16-bit library
+// product here; in a long run the 1000 W limit leaves 2.8).
 constexpr unsigned kPairSlices = 2;
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, unsigned bar, int x, int y) {
@@ -579,6 +484,7 @@ __device__ __forceinline__ void mma_commit_pair(unsigned long long* bar) {
 __device__ __forceinline__ void arrive_at(unsigned bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+
 __global__ void __launch_bounds__(kTcThreads, 1)
 matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__ CUtensorMap amap, const TcArgs g) {
     extern __shared__ unsigned char smem_raw[];
@@ -717,37 +623,30 @@ CUtensorMap slice_map(const signed char* p, unsigned rows, unsigned k, unsigned 
     return map;
 }
 
-void launch_tc(const MatmulQ8Args& a, bool pair) {
+// Stages take up to 220 KB; 1 KB more aligns them.
+constexpr int kTcSmem = 222 * 1024;
+
+void launch_pair(const MatmulQ8Args& a) {
     TcArgs g{};
     g.sa = a.sa, g.sb = a.sb, g.bias = a.bias, g.out = a.out, g.m = a.m, g.n = a.n;
     g.err = device_error_word();
-    const unsigned step = pair ? 32 : 16;
-    g.bn = std::min(256u, (a.m + step - 1) / step * step);
-    const unsigned slices = pair ? kPairSlices : 1;
-    g.steps = (a.k + slices * kSliceK - 1) / (slices * kSliceK);
-    const unsigned tile_n = pair ? 2 * kTileM : kTileM;
+    g.bn = std::min(256u, (a.m + 31) / 32 * 32);
+    g.steps = (a.k + kPairSlices * kSliceK - 1) / (kPairSlices * kSliceK);
     g.tiles_m = (a.m + g.bn - 1) / g.bn;
-    g.tiles_n = (a.n + tile_n - 1) / tile_n;
-    const unsigned tokens = pair ? g.bn / 2 : g.bn;  // a CTA fetches
-    const unsigned stage = slices * (kTileM + tokens) * kSliceK;
+    g.tiles_n = (a.n + 2 * kTileM - 1) / (2 * kTileM);
+    const unsigned stage = kPairSlices * (kTileM + g.bn / 2) * kSliceK;  // in each CTA
     g.stages = std::min(8u, 220u * 1024 / stage);
     g.tmem_cols = 32;
     while (g.tmem_cols < 2 * g.bn) g.tmem_cols *= 2;
     // 32-bit integer accumulators, signed 8-bit sides, both K-major
-    g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (tile_n >> 4) << 24;
+    g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (2 * kTileM >> 4) << 24;
     if (static_cast<unsigned long long>(g.tiles_m) * g.tiles_n > 0x7fffffffull)
         fail(VC_ERR_OVERFLOW, "matmul_q8: too many tiles");
-    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, tokens);
-    constexpr unsigned kMaxSmem = 222 * 1024;
-    static bool configured = false;
-    if (!configured) {
-        VC_CUDA(cudaFuncSetAttribute(matmul_q8_tc, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-        VC_CUDA(cudaFuncSetAttribute(matmul_q8_pair, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-        configured = true;
-    }
+    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn / 2);
+    allow_smem<matmul_q8_pair, kTcSmem>();
     const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(pair ? 2 * std::min(ntiles, sms / 2) : std::min(ntiles, sms));
+    cfg.gridDim = dim3(2 * std::min(ntiles, sms / 2));
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = g.stages * stage + 1024;
     cfg.stream = stream();
@@ -756,12 +655,13 @@ void launch_tc(const MatmulQ8Args& a, bool pair) {
     attr[0].val.clusterDim.x = 2;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = pair ? 1 : 0;
-    VC_CUDA(cudaLaunchKernelEx(&cfg, pair ? matmul_q8_pair : matmul_q8_tc, bmap, amap, g));
-    check_launch("matmul_q8_tc");
+    cfg.numAttrs = 1;
+    VC_CUDA(cudaLaunchKernelEx(&cfg, matmul_q8_pair, bmap, amap, g));
+    check_launch("matmul_q8_pair");
 }
 
-// The least steps along k that are worth a CTA of their own.
+// The least steps along k that are worth a CTA of their own (with 2 or 8 the
+// sizes above run the same within 1%).
 constexpr unsigned kSplitSteps = 4;
 
 void launch_split(const MatmulQ8Args& a) {
@@ -778,7 +678,7 @@ void launch_split(const MatmulQ8Args& a) {
     const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
     g.stages = std::min(8u, 220u * 1024 / stage);
     p.split = 1;
-    while (p.split < 8 && 2 * p.split * ntiles <= sms && g.steps >= 2 * p.split * kSplitSteps) p.split *= 2;
+    while (p.split < 4 && 2 * p.split * ntiles <= sms && g.steps >= 2 * p.split * kSplitSteps) p.split *= 2;
     p.part = (g.steps + p.split - 1) / p.split;
     while (p.split > 1 && (p.split - 1) * p.part >= g.steps) p.split /= 2, p.part = (g.steps + p.split - 1) / p.split;
     g.tmem_cols = 32;
@@ -787,12 +687,7 @@ void launch_split(const MatmulQ8Args& a) {
     p.sums = sums.as<int>();
     g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (kTileM >> 4) << 24;
     const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn);
-    constexpr unsigned kMaxSmem = 222 * 1024;
-    static bool configured = false;
-    if (!configured) {
-        VC_CUDA(cudaFuncSetAttribute(matmul_q8_split, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem));
-        configured = true;
-    }
+    allow_smem<matmul_q8_split, kTcSmem>();
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ntiles * p.split);
     cfg.blockDim = dim3(kTcThreads);
@@ -839,12 +734,19 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
     if (k == 0) {
         matmul_q8_empty<<<grid_for(m * n, 256), 256, 0, stream()>>>(a_scale, b_scale, bias, g.m, g.n, out);
         check_launch("matmul_q8_empty");
-    } else if (m <= kRowsTokens) {
-        launch_rows(g);
-    } else if (2 * ((n + kTileM - 1) / kTileM) * ((m + 255) / 256) <= static_cast<size_t>(sm_count())) {
-        launch_split(g);
     } else {
-        launch_tc(g, m > 128);
+        // Tiles of 128 weight rows and up to 256 tokens, against the SMs (all in
+        // us, k = 4096): below half of them a tile is shared (64 x 4096: 10.9,
+        // in pairs 13.3; 200 x 8192, at half: 18.2 and 17.9), else pairs walk the
+        // tiles (64 x 11008: 15.0, one CTA a tile 15.9; 4096 x 4096: 54 and 79).
+        // Up to 8 tokens the weights go straight to registers (8 x 32000: 26, in
+        // pairs 30), up to 16 while the tiles are few (16 x 4096: 6.8, shared
+        // 8.3; 16 x 32000 the other way, 33 and 30).
+        const size_t sms = static_cast<size_t>(sm_count());
+        const size_t tiles = ((n + kTileM - 1) / kTileM) * ((m + 255) / 256);
+        if (m <= 8 || (m <= 16 && tiles <= sms)) launch_rows(g);
+        else if (2 * tiles <= sms) launch_split(g);
+        else launch_pair(g);
     }
     VC_API_END
 }

@@ -721,6 +721,12 @@ norm_bwd_ring(const RingArgs a) {
     }
 }
 
+template <int NV>
+void launch_ring(const RingArgs& a, unsigned ctas, unsigned smem) {
+    allow_smem<norm_bwd_ring<NV>, kRingSmem>();
+    norm_bwd_ring<NV><<<ctas, kRingThreads + 32, smem, stream()>>>(a);
+}
+
 // The fused pass, where it applies; false, having launched nothing, otherwise.
 bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
     if (n.cols % 4 != 0 || n.cols > kRingCols || !aligned16(n.h) || !aligned16(n.gy) || !aligned16(n.w) ||
@@ -742,14 +748,10 @@ bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
     Scratch partial(partial_rows * n.cols * sizeof(float));
     a.partial = partial.as<float>();
     a.err = device_error_word();
-    const auto launch = [&](auto kernel) {
-        VC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingSmem));
-        kernel<<<sms, kRingThreads + 32, a.stages * stage, stream()>>>(a);
-    };
     const unsigned per = (n.cols / 4 + a.T - 1) / a.T;
-    if (per <= 1) launch(norm_bwd_ring<1>);
-    else if (per <= 2) launch(norm_bwd_ring<2>);
-    else launch(norm_bwd_ring<4>);
+    if (per <= 1) launch_ring<1>(a, sms, a.stages * stage);
+    else if (per <= 2) launch_ring<2>(a, sms, a.stages * stage);
+    else launch_ring<4>(a, sms, a.stages * stage);
     check_launch("norm_bwd_ring");
     launch_dw_finish(a.partial, partial_rows, n.cols, dw);
     return true;
@@ -795,6 +797,13 @@ void check_q8_out(const char* what, const void* q, const float* scale, std::size
                                                  "multiple of 16 bytes, on a 16-byte aligned base");
 }
 
+// h may be the very tensor it is computed from, where row i of both is the same memory.
+void check_in_place(const char* what, const float* h, const float* from, std::size_t stride, std::size_t rows,
+                    std::size_t cols) {
+    if (h && h == from && stride != cols && rows > 1)
+        fail(VC_ERR_INVALID, std::string(what) + ": h can be written over a contiguous tensor only");
+}
+
 void check_eps(const char* what, float eps) {
     if (!(eps >= 0.0f) || !std::isfinite(eps)) fail(VC_ERR_INVALID, std::string(what) + ": eps must be finite and not negative");
 }
@@ -815,6 +824,8 @@ vc_status vc_cuda_rms_norm(const float* x, size_t x_stride, const float* residua
     check_eps("rms_norm", eps);
     if (rows == 0) return VC_OK;
     if (!x || !weight || !y) fail(VC_ERR_INVALID, "rms_norm: null pointer");
+    check_in_place("rms_norm", h, x, x_stride, rows, cols);
+    check_in_place("rms_norm", h, residual, residual_stride, rows, cols);
     NormArgs a{};
     a.x = x, a.xs = x_stride, a.r = residual, a.rs = residual_stride, a.w = weight;
     a.rows = rows, a.cols = static_cast<unsigned>(cols), a.eps = eps;
@@ -832,6 +843,8 @@ vc_status vc_cuda_rms_norm_q8(const float* x, size_t x_stride, const float* resi
     check_eps("rms_norm_q8", eps);
     if (rows == 0) return VC_OK;
     if (!x || !weight) fail(VC_ERR_INVALID, "rms_norm_q8: null pointer");
+    check_in_place("rms_norm_q8", h, x, x_stride, rows, cols);
+    check_in_place("rms_norm_q8", h, residual, residual_stride, rows, cols);
     check_q8_out("rms_norm_q8", q, scale, cols, q_pitch);
     NormArgs a{};
     a.x = x, a.xs = x_stride, a.r = residual, a.rs = residual_stride, a.w = weight;

@@ -213,6 +213,16 @@ inline void launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, std::siz
     if (err != cudaSuccess) throw std::runtime_error(std::string("cudaLaunchKernelEx: ") + cudaGetErrorString(err));
 }
 
+// Lets a kernel take up to BYTES of dynamic shared memory; once a process.
+template <auto KERNEL, int BYTES>
+inline void allow_smem() {
+    static const bool done = [] {
+        VC_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+        return true;
+    }();
+    (void)done;
+}
+
 __device__ __forceinline__ unsigned smem_addr(const void* p) {
     return static_cast<unsigned>(__cvta_generic_to_shared(p));
 }
