@@ -19,16 +19,20 @@
 // winner among all classes is drawn, the mass ahead of it added up, and with
 // probability p that is below p of the whole and the row is done; else the race
 // is run again among the classes ahead of it. Sums are added in a fixed order
-// (four weights in float, then in double), so nothing depends on scheduling.
+// (up to eight weights in float, then in double), those over lists in whole
+// multiples of 2^-40, so nothing depends on scheduling.
 //
-// A small k has its classes listed and sorted: none of them is below the k-th
-// largest of the maxima of some 2k groups of threads. A large k, or more equal
-// logits than the list holds, has its last class found by five histograms of the
-// order's key, (ordered logit bits, ~index), 11 bits each.
+// Few classes are left by a small k or by min-p, so these are listed on the way
+// and the rest of the work is the list's. None of the top k is below the k-th
+// largest of the maxima of some 2k groups of threads: the classes from there on
+// go to the row's first CTA, which sorts them. The ones that reach min-p stay with
+// their CTA, unless they are too many. A large k, or more equal logits than the
+// sorted list holds, has its last class found by up to five histograms of the
+// order's key, (ordered logit bits, ~index), 11 bits each, and then a list too.
 //
 // Without top-k and min-p a row is read once from HBM, the sum and the race
-// running against the maximum so far; with them, once for its maximum. What
-// follows reads it from L1 or L2.
+// running against the maximum so far; with them, once for its maximum and once,
+// from L1 or L2, for the sum and the list.
 //
 // Weights come in two makes. `weight` is the definition in float: one
 // subtraction, one division, expf. `quick` is one product and ex2.approx,
@@ -50,7 +54,9 @@ namespace cg = cooperative_groups;
 using u64 = unsigned long long;
 
 constexpr unsigned kBins = 2048;       // of a histogram
-constexpr unsigned kSorted = 512;      // classes a sorted list holds, over the cluster
+template <unsigned THREADS>
+constexpr unsigned kList = THREADS < 512 ? 2048 : 4096;  // classes a CTA lists
+constexpr unsigned kSorted = 512;      // classes that are sorted, of the whole cluster
 constexpr unsigned kGroups = 512;      // of threads, over the cluster, whose maxima bound the top k
 constexpr unsigned kMaxWarps = 32;
 constexpr unsigned kIndexBits = 23;    // a key is 32 ordered logit bits, then these of ~index
@@ -141,18 +147,17 @@ struct Weigh {
 
 struct Shared {
     unsigned count[kBins];
-    u64 pick[kSorted], sorted[kSorted];
+    u64 pick[kSorted];          // in the first CTA, of the whole cluster
     float4 group[kGroups / 4];  // maxima of groups of threads, over the cluster
-    float cut;
+    float kth;
     u64 warp64[kMaxWarps];
     double warpd[kMaxWarps];
-    unsigned picked;
-    unsigned found_bin;  // kBins: none
+    unsigned listed, picked;
+    unsigned found_bin, found_in;  // kBins: none
     u64 found_ahead;
     // written by every CTA of the cluster, by its rank
     u64 top[kMaxCluster], best[2][kMaxCluster];
     double total[kMaxCluster], mass[2][kMaxCluster];
-    unsigned in_pick[kMaxCluster];
     u64 share[kMaxCluster];
 };
 
@@ -417,15 +422,16 @@ struct Race {
     }
     __device__ __forceinline__ u64 best(const Weigh& wt) const { return leader == 0xffffffffu ? 0 : exact(wt, leader); }
 
-    // The random numbers of a quad's classes with a weight, 16 bytes a load
-    // where the row allows it (a loose class has no neighbours).
-    __device__ __forceinline__ float4 numbers(const float4& w, unsigned i, bool even) const {
+    // The random numbers of the classes from i on, as many as there are before
+    // `end`, 16 bytes a load where the row allows it.
+    __device__ __forceinline__ float4 numbers(unsigned i, unsigned end, bool loose) const {
         float4 e = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-        if (even && w.y + w.z + w.w > 0.0f) return *reinterpret_cast<const float4*>(noise + i);
-        if (w.x > 0.0f) e.x = noise[i];
-        if (w.y > 0.0f) e.y = noise[i + 1];
-        if (w.z > 0.0f) e.z = noise[i + 2];
-        if (w.w > 0.0f) e.w = noise[i + 3];
+        if (loose) {
+            if (i < end) e.x = noise[i];
+        } else if (i + 3 < end) {
+            if ((reinterpret_cast<std::uintptr_t>(noise + i) & 15) == 0) return *reinterpret_cast<const float4*>(noise + i);
+            e = make_float4(noise[i], noise[i + 1], noise[i + 2], noise[i + 3]);
+        }
         return e;
     }
 };
@@ -437,6 +443,7 @@ struct Race {
 struct Found {
     unsigned bin;
     u64 ahead;
+    unsigned in_bin;
 };
 __device__ __noinline__ Found find_bin(Shared& s, u64 target) {
     const cg::cluster_group cluster = cg::this_cluster();
@@ -471,45 +478,80 @@ __device__ __noinline__ Found find_bin(Shared& s, u64 target) {
         for (unsigned r = 0; r < rank; ++r) c += s.share[r];
     }
     if (any && c < target && c + mine >= target) {
-        unsigned j = 0;
+        unsigned j = 0, in_bin = n[0];
 #pragma unroll
         for (unsigned i = 0; i < 7; ++i)
-            if (j == i && c + n[i] < target) c += n[i], ++j;
+            if (j == i && c + n[i] < target) c += n[i], in_bin = n[i + 1], ++j;
         for (unsigned r = 0; r < C; ++r) {
             Shared* o = cluster.map_shared_rank(&s, r);
             o->found_bin = first + j;
             o->found_ahead = c;
+            o->found_in = in_bin;
         }
     }
     row_sync(cluster);
-    return Found{s.found_bin, s.found_ahead};
+    return Found{s.found_bin, s.found_ahead, s.found_in};
 }
 
-// The classes picked by the CTAs of the cluster (n of them, counts in in_pick),
-// in the first CTA's `sorted`, largest first: a warp fetches each CTA's, then
-// every class counts the ones before it -- one barrier, where a sorting network
-// of 256 has 36.
-__device__ __noinline__ void sort_picks(Shared& s, unsigned n) {
-    const cg::cluster_group cluster = cg::this_cluster();
-    const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp > 0 && warp < cluster.num_blocks()) {
-        unsigned at = 0;
-        for (unsigned r = 0; r < warp; ++r) at += s.in_pick[r];
-        const Shared* o = cluster.map_shared_rank(&s, warp);
-        for (unsigned i = lane; i < s.in_pick[warp]; i += 32) s.pick[at + i] = o->pick[i];
-    }
-    __syncthreads();
-    for (unsigned c = threadIdx.x; c < n; c += blockDim.x) {
-        const u64 mine = s.pick[c];
+// The k-th largest of n numbers, a power of two from 8 to kGroups: each is told its
+// place by the threads that compare it with all, as many threads a number as there are.
+template <unsigned THREADS>
+__device__ __noinline__ float kth_of(Shared& s, const float4* v, unsigned n, unsigned k) {
+    unsigned per = 1;
+    while (per < 32 && 2 * per * n <= THREADS && 8 * per <= n) per *= 2;
+    const unsigned part = threadIdx.x % per;
+    for (unsigned base = 0; base < n; base += THREADS / per) {
+        const unsigned g = base + threadIdx.x / per;
+        const float mine = reinterpret_cast<const float*>(v)[min(g, n - 1)];
         unsigned place = 0;
 #pragma unroll 4
-        for (unsigned i = 0; i < n; ++i) place += s.pick[i] > mine;
-        s.sorted[place] = mine;
+        for (unsigned q = part; q < n / 4; q += per) {
+            const float4 o = v[q];
+            const unsigned i = 4 * q;
+            place += (o.x > mine || (o.x == mine && i < g)) + (o.y > mine || (o.y == mine && i + 1 < g)) +
+                     (o.z > mine || (o.z == mine && i + 2 < g)) + (o.w > mine || (o.w == mine && i + 3 < g));
+        }
+        for (unsigned m = 1; m < per; m <<= 1) place += __shfl_xor_sync(0xffffffffu, place, m);
+        if (g < n && place == k - 1) s.kth = mine;
+    }
+    __syncthreads();
+    return s.kth;
+}
+
+// Groups a warp, so that there are 2k over all warps if there can be.
+__device__ __forceinline__ unsigned groups_a_warp(unsigned warps, u64 k) {
+    unsigned per = 1;
+    while (per < 32 && 2 * per * warps <= kGroups && per * warps < 2 * k) per *= 2;
+    return per;
+}
+// The maximum of the group of lanes, `per` groups a warp.
+__device__ __forceinline__ float group_max(float v, unsigned per) {
+    for (unsigned m = 1; m < 32 / per; m <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, m));
+    return v;
+}
+
+// The n classes of s.pick in order, largest first, in `sorted`, and their random
+// numbers: every class counts the ones before it, shared by as many
+// threads as there are -- one barrier, where a sorting network of 256 has 36.
+template <unsigned THREADS>
+__device__ __noinline__ void sort_picks(const Shared& s, unsigned n, const float* noise, u64* sorted, float* numbers) {
+    unsigned per = 1;
+    while (per < 32 && 2 * per * n <= THREADS) per *= 2;
+    const unsigned part = threadIdx.x % per;
+    for (unsigned base = 0; base < n; base += THREADS / per) {
+        const unsigned c = base + threadIdx.x / per;
+        const u64 mine = s.pick[min(c, n - 1)];
+        const float e = part == 0 ? noise[key_index(mine)] : 0.0f;
+        unsigned place = 0;
+#pragma unroll 4
+        for (unsigned i = part; i < n; i += per) place += s.pick[i] > mine;
+        for (unsigned m = 1; m < per; m <<= 1) place += __shfl_xor_sync(0xffffffffu, place, m);
+        if (c < n && part == 0) sorted[place] = mine, numbers[place] = e;
     }
     __syncthreads();
 }
 
-// The key of the k-th class in order (k at most the classes in play).
+// A key that k classes reach and no more; the lowest if no more than k are in play.
 template <unsigned THREADS>
 __device__ __noinline__ u64 kth_key(Shared& s, const float* x, unsigned begin, unsigned end, u64 k) {
     u64 prefix = 0;
@@ -526,9 +568,10 @@ __device__ __noinline__ u64 kth_key(Shared& s, const float* x, unsigned begin, u
             tally(v.x, i), tally(v.y, i + 1), tally(v.z, i + 2), tally(v.w, i + 3);
         });
         const Found f = find_bin(s, k);
-        if (f.bin == kBins) return 0;  // fewer than k classes: all stay
+        if (f.bin == kBins) return key_of(-INFINITY, kIndexMask);  // fewer than k classes: all stay
         k -= f.ahead;
         prefix = prefix << kLevelBits | (kBins - 1 - f.bin);
+        if (k == f.in_bin) return prefix << shift;  // the bin's classes are the last of the k
     }
     return prefix;
 }
@@ -550,6 +593,8 @@ template <unsigned THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_kernel(const SampleArgs a) {
     __shared__ Shared s;
+    // the keys of the classes that may be left; later the sorted ones, with their numbers
+    __shared__ u64 list[kList<THREADS>];
     const cg::cluster_group cluster = cg::this_cluster();
     const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
     const u64 row = blockIdx.x / C;
@@ -577,32 +622,27 @@ sample_kernel(const SampleArgs a) {
     double total = 0.0;
     float own_peak = -INFINITY;  // this thread's
     // Races the classes of the row that `joins(quad, index, weights)` leaves a
-    // weight: their random numbers are fetched together before any is looked at.
-    // The best of each thread's first classes is known beforehand, so that few of
-    // the rest have to be compared one by one.
+    // weight. The best of each thread's first classes is known beforehand, so that
+    // few of the rest have to be compared one by one.
     const auto race_those = [&](auto&& joins) {
         {
             const First f = first_quad(x, begin, end);
+            const float4 e = race.numbers(f.i, end, false);
             float4 w = wt.quick(f.v);
-            const double kept = total;
             joins(f.v, f.i, w);
-            total = kept;  // the pass below adds these too
-            const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + f.i) & 15) == 0;
-            const float score = largest(w) > 0.0f ? largest(race.scores(w, race.numbers(w, f.i, even))) : 0.0f;
-            race.start_from(fmaxf(block_max_f(score, s), 0.0f));
+            race.start_from(fmaxf(block_max_f(largest(race.scores(w, e)), s), 0.0f));
         }
         each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
             constexpr int quads = sizeof(v) / sizeof(float4);
-            const bool even = !decltype(loose)::value && (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
             float4 w[quads], e[quads];
+#pragma unroll
+            for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, decltype(loose)::value);
 #pragma unroll
             for (int j = 0; j < quads; ++j) {
                 w[j] = wt.quick(v[j]);
                 joins(v[j], first + j * 4 * THREADS, w[j]);
             }
             if (!__any_sync(0xffffffffu, largest(w) > 0.0f)) return;
-#pragma unroll
-            for (int j = 0; j < quads; ++j) e[j] = race.numbers(w[j], first + j * 4 * THREADS, even);
             race.template run<THREADS>(wt, w, e, first);
         });
     };
@@ -610,30 +650,16 @@ sample_kernel(const SampleArgs a) {
     if (at_once) {
         // one pass: the sum and the race relative to the warp's maximum so far
         const First f = first_quad(x, begin, end);
+        const float4 e = first_only ? f.v : race.numbers(f.i, end, false);
         wt.m = fmaxf(capped(block_max_f(largest(f.v), s)), -kLargest);  // no class in play is below that
-        if (!first_only) {
-            const float4 w = wt.quick(f.v);
-            const bool even = (reinterpret_cast<std::uintptr_t>(race.noise + f.i) & 15) == 0;
-            const float score = largest(w) > 0.0f ? largest(race.scores(w, race.numbers(w, f.i, even))) : 0.0f;
-            race.start_from(fmaxf(block_max_f(score, s), 0.0f));
-        }
+        if (!first_only) race.start_from(fmaxf(block_max_f(largest(race.scores(wt.quick(f.v), e)), s), 0.0f));
+        peak.high = wt.m == 0.0f ? -0x1p-149f : from_ordered(ordered(wt.m) - 1);  // what reaches that maximum is of interest
         each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
             constexpr int quads = sizeof(v) / sizeof(float4);
             float4 w[quads], e[quads];
-            const bool even = !decltype(loose)::value && (reinterpret_cast<std::uintptr_t>(race.noise + first) & 15) == 0;
+            if (!first_only)
 #pragma unroll
-            for (int j = 0; j < quads; ++j) {
-                const unsigned i = first + j * 4 * THREADS;
-                e[j] = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-                if (first_only) continue;
-                if constexpr (decltype(loose)::value) {
-                    if (i < end) e[j].x = race.noise[i];
-                } else if (quads > 1 || i + 3 < end) {  // a quad of the row, not past its last
-                    if (even) e[j] = *reinterpret_cast<const float4*>(race.noise + i);
-                    else
-                        e[j] = make_float4(race.noise[i], race.noise[i + 1], race.noise[i + 2], race.noise[i + 3]);
-                }
-            }
+                for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, decltype(loose)::value);
             peak.template see<THREADS>(v, first, loose);
             if (peak.high > wt.m) {  // the whole warp
                 const float less = exp2_quick((wt.m - peak.high) * wt.to_log2);
@@ -655,21 +681,18 @@ sample_kernel(const SampleArgs a) {
     u64 top = 0;
     if (peak.at != 0xffffffffu) top = key_of(peak.high < kLargest ? peak.high : x[peak.at], peak.at);
     top = block_max64(top, s);
-    if (t == 0) s.picked = 0;
+    if (t == 0) s.listed = s.picked = 0;
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
     // the maxima of groups of neighbouring threads, 2k groups if there are as many
     const bool few = k && k <= kSorted / 2;
     const unsigned warps = C * THREADS / 32;  // of the cluster, at most 256
-    unsigned per_warp = 1;                    // groups
+    const unsigned per_warp = groups_a_warp(warps, k), groups = warps * per_warp;
     if (few) {
-        while (per_warp < 32 && 2 * per_warp * warps <= kGroups && per_warp * warps < 2 * k) per_warp *= 2;
-        float high = own_peak;
-        for (unsigned m = 1; m < 32 / per_warp; m <<= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, m));
-        const unsigned lanes = 32 / per_warp, lane = t & 31;
-        if (lane % lanes == 0)
+        const unsigned lanes = 32 / per_warp;
+        const float high = group_max(own_peak, per_warp);
+        if (t % lanes == 0)
             for (unsigned r = 0; r < C; ++r)
-                reinterpret_cast<float*>(cluster.map_shared_rank(&s, r)->group)[(rank * THREADS / 32 + (t >> 5)) * per_warp +
-                                                                              lane / lanes] = high;
+                reinterpret_cast<float*>(cluster.map_shared_rank(&s, r)->group)[(rank * THREADS + t) / lanes] = high;
     }
     tell_all(cluster, s, [&](Shared& o) { o.top[rank] = top; });
     row_sync(cluster);
@@ -685,148 +708,185 @@ sample_kernel(const SampleArgs a) {
     if (at_once) total *= exp2_quick((wt.m - high) * wt.to_log2);
     wt.m = high;
 
-    // A small k: the k-th largest of the groups' maxima is a lower bound of the top k.
-    bool listing = false;
-    float list_from = -INFINITY;
-    const unsigned groups = warps * per_warp;
-    if (few && k <= groups) {
-        for (unsigned g = t; g < groups; g += THREADS) {
-            const float mine = reinterpret_cast<const float*>(s.group)[g];
-            unsigned place = 0;
-#pragma unroll 4
-            for (unsigned i = 0; i < groups; i += 4) {
-                const float4 o = s.group[i / 4];
-                place += (o.x > mine || (o.x == mine && i < g)) + (o.y > mine || (o.y == mine && i + 1 < g)) +
-                         (o.z > mine || (o.z == mine && i + 2 < g)) + (o.w > mine || (o.w == mine && i + 3 < g));
-            }
-            if (place == k - 1) s.cut = mine;
-        }
-        __syncthreads();
-        list_from = s.cut;
-        listing = in_play(list_from);
-    }
-    // The row's sum, and with it the list, or the race of the classes that min-p
-    // leaves.
-    if (k) {
+    // The classes that may be left are listed: of a small k, from the k-th largest
+    // of the groups' maxima on, and by the first CTA; of min-p, the ones that reach
+    // it, each CTA its own.
+    float cut = -INFINITY;
+    if (few && k <= groups) cut = kth_of<THREADS>(s, s.group, groups, static_cast<unsigned>(k));
+    const bool picking = in_play(cut), listing = min_p > 0.0f && !k;
+    if (picking) {
+        Shared* one = cluster.map_shared_rank(&s, 0);
         each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
             total += sum4(wt.quick(v));
-            if (!listing || !(largest(v) >= list_from)) return;
-            const auto lists = [&](float u, unsigned j) {
-                if (u >= list_from && in_play(u)) {
-                    const unsigned at = atomicAdd(&s.picked, 1u);
-                    if (at < kSorted) s.pick[at] = key_of(u, j);
+            if (!(largest(v) >= cut)) return;
+            const auto picks = [&](float u, unsigned j) {
+                if (u >= cut && in_play(u)) {
+                    const unsigned at = atomicAdd(&one->picked, 1u);
+                    if (at < kSorted) one->pick[at] = key_of(u, j);
                 }
             };
-            lists(v.x, i), lists(v.y, i + 1), lists(v.z, i + 2), lists(v.w, i + 3);
+            picks(v.x, i), picks(v.y, i + 1), picks(v.z, i + 2), picks(v.w, i + 3);
         });
     } else if (!at_once) {
-        race_those([&](const float4& v, unsigned, float4& w) {
+        float least = listing ? min_p * (1.0f - kNear) : INFINITY;
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+            const float4 w = wt.quick(v);
             total += sum4(w);
-            if (!wt.reaches(min_p, w.x, v.x)) w.x = 0.0f;
-            if (!wt.reaches(min_p, w.y, v.y)) w.y = 0.0f;
-            if (!wt.reaches(min_p, w.z, v.z)) w.z = 0.0f;
-            if (!wt.reaches(min_p, w.w, v.w)) w.w = 0.0f;
+            if (!(largest(w) >= least)) return;
+            const auto lists = [&](float u, float w, unsigned j) {
+                if (w >= least && wt.reaches(min_p, w, u)) {
+                    const unsigned at = atomicAdd(&s.listed, 1u);
+                    if (at < kList<THREADS>) list[at] = key_of(u, j);
+                    else least = INFINITY;  // the list is full
+                }
+            };
+            lists(v.x, w.x, i), lists(v.y, w.y, i + 1), lists(v.z, w.z, i + 2), lists(v.w, w.w, i + 3);
         });
     }
     total = block_sum_d(total, s);
-    tell_all(cluster, s, [&](Shared& o) {
-        o.total[rank] = total;
-        o.in_pick[rank] = s.picked;
-    });
+    tell_all(cluster, s, [&](Shared& o) { o.total[rank] = total; });
     const auto over_cluster = [&](const double* parts) {
         double all = 0.0;
         for (unsigned r = 0; r < C; ++r) all += parts[r];
         return all;
     };
+    const auto answer = [&](u64 won) {
+        if (rank != 0 || t != 0) return;
+        const unsigned token = won == 0 ? key_index(top) : ~static_cast<unsigned>(won);
+        a.token[row] = token;
+        a.logprob[row] = wt.distance(x[token]) - logf(static_cast<float>(over_cluster(s.total)));
+    };
+
+    if (picking) {
+        row_sync(cluster);
+        const unsigned picked = cluster.map_shared_rank(&s, 0)->picked;
+        if (picked <= kSorted) {
+            if (rank != 0) return;
+            // the classes in order, `per` a thread: the filters, then the race of the ones left
+            constexpr unsigned per = kSorted > THREADS ? kSorted / THREADS : 1;
+            float* numbers = reinterpret_cast<float*>(list + kSorted);
+            sort_picks<THREADS>(s, picked, race.noise, list, numbers);
+            u64 key[per], mass[per], sum = 0, best = 0;
+            float w[per];
+#pragma unroll
+            for (unsigned j = 0; j < per; ++j) {
+                const unsigned at = t * per + j;
+                key[j] = at < picked && at < k ? list[at] : 0;
+                w[j] = key[j] ? wt.quick(key_logit(key[j])) : 0.0f;
+                mass[j] = __float2ull_rn(w[j] * 0x1p40f);  // whole numbers: exact sums in any order
+                sum += mass[j];
+            }
+            const Scan scan = block_scan(sum, s);
+            u64 before = scan.before;
+            const double most = static_cast<double>(p_in) * static_cast<double>(scan.all);
+#pragma unroll
+            for (unsigned j = 0; j < per; ++j) {
+                const float v = key_logit(key[j]);
+                if (key[j] && (!by_p || static_cast<double>(before) < most) && wt.reaches(min_p, w[j], v))
+                    best = max(best, exact_score(v, numbers[t * per + j], key_index(key[j]), wt.m, wt.t));
+                before += mass[j];
+            }
+            answer(block_max64(best, s));
+            if (C > 1) cluster.sync();  // the others have left, or read `picked` first
+            return;
+        }
+    }
+
+    unsigned turn = 0;  // of the slots that go round
     const auto mass_of_all = [&](double mine, unsigned turn) {
         mine = block_sum_d(mine, s);
         tell_all(cluster, s, [&](Shared& o) { o.mass[turn & 1][rank] = mine; });
         row_sync(cluster);
         return over_cluster(s.mass[turn & 1]);
     };
-    unsigned turn = 0;  // of the slots that go round
-    bool sorted = false;
-    u64 listed_best = 0;  // of the sorted classes
+    // Whether this CTA has a list of every class that may be left.
+    const bool by_list = k ? k <= kList<THREADS> : listing && s.listed <= kList<THREADS>;
+    u64 best = 0;
+    const auto race_listed = [&](auto&& joins) {
+        constexpr unsigned per = kList<THREADS> / THREADS;
+        float e[per];
+        best = 0;
+#pragma unroll
+        for (unsigned j = 0; j < per; ++j)
+            if (t + j * THREADS < s.listed) e[j] = race.noise[key_index(list[t + j * THREADS])];
+#pragma unroll
+        for (unsigned j = 0; j < per; ++j) {
+            if (t + j * THREADS >= s.listed) break;
+            const u64 key = list[t + j * THREADS];
+            const float u = key_logit(key);
+            if (joins(u, key_index(key))) best = max(best, exact_score(u, e[j], key_index(key), wt.m, wt.t));
+        }
+    };
     double limit = 0.0;
     if (k) {
-        row_sync(cluster);
-        unsigned n = 0;
-        for (unsigned r = 0; r < C; ++r) n += s.in_pick[r];
-        sorted = listing && n <= kSorted;
-        if (sorted) {
-            if (rank == 0) {
-                // the classes in order, `per` a thread: the filters, then the race of the ones left
-                constexpr unsigned per = kSorted > THREADS ? kSorted / THREADS : 1;
-                sort_picks(s, n);
-                u64 key[per], mass[per], sum = 0;
-                float w[per], e[per];
-#pragma unroll
-                for (unsigned j = 0; j < per; ++j) {
-                    const unsigned at = t * per + j;
-                    key[j] = at < n && at < k ? s.sorted[at] : 0;
-                    w[j] = key[j] ? wt.quick(key_logit(key[j])) : 0.0f;
-                    e[j] = key[j] ? race.noise[key_index(key[j])] : 1.0f;
-                    mass[j] = __float2ull_rn(w[j] * 0x1p40f);  // whole numbers: exact sums in any order
-                    sum += mass[j];
-                }
-                const Scan scan = block_scan(sum, s);
-                u64 before = scan.before;
-                const double most = static_cast<double>(p_in) * static_cast<double>(scan.all);
-#pragma unroll
-                for (unsigned j = 0; j < per; ++j) {
-                    const float v = key_logit(key[j]);
-                    if (key[j] && (!by_p || static_cast<double>(before) < most) && wt.reaches(min_p, w[j], v))
-                        listed_best = max(listed_best, exact_score(v, e[j], key_index(key[j]), wt.m, wt.t));
-                    before += mass[j];
-                }
-            }
+        const u64 least = kth_key<THREADS>(s, x, begin, end, k);
+        double mass = 0.0;
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+            if (!(largest(v) >= key_logit(least))) return;
+            const auto keep = [&](float u, unsigned j) {
+                if (!in_play(u) || key_of(u, j) < least) return 0.0f;
+                if (by_list) list[atomicAdd(&s.listed, 1u)] = key_of(u, j);
+                return wt.quick(u);
+            };
+            mass += sum4(make_float4(keep(v.x, i), keep(v.y, i + 1), keep(v.z, i + 2), keep(v.w, i + 3)));
+        });
+        limit = static_cast<double>(p_in) * mass_of_all(mass, turn++);
+        if (by_list) {
+            race_listed([&](float u, unsigned) { return wt.reaches(min_p, wt.quick(u), u); });
         } else {
-            const u64 least = kth_key<THREADS>(s, x, begin, end, k);
-            double mass = 0.0;
-            each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
-                const auto keep = [&](float u, unsigned j) {
-                    return in_play(u) && key_of(u, j) >= least ? wt.quick(u) : 0.0f;
-                };
-                mass += sum4(make_float4(keep(v.x, i), keep(v.y, i + 1), keep(v.z, i + 2), keep(v.w, i + 3)));
-            });
             race_those([&](const float4& v, unsigned i, float4& w) {
                 const auto keep = [&](float u, unsigned j, float& w) {
                     if (!in_play(u) || key_of(u, j) < least || !wt.reaches(min_p, w, u)) w = 0.0f;
                 };
                 keep(v.x, i, w.x), keep(v.y, i + 1, w.y), keep(v.z, i + 2, w.z), keep(v.w, i + 3, w.w);
             });
-            limit = static_cast<double>(p_in) * mass_of_all(mass, turn++);
         }
+    } else if (by_list) {
+        race_listed([](float, unsigned) { return true; });
+    } else if (!at_once) {
+        race_those([&](const float4& v, unsigned, float4& w) {
+            if (!wt.reaches(min_p, w.x, v.x)) w.x = 0.0f;
+            if (!wt.reaches(min_p, w.y, v.y)) w.y = 0.0f;
+            if (!wt.reaches(min_p, w.z, v.z)) w.z = 0.0f;
+            if (!wt.reaches(min_p, w.w, v.w)) w.w = 0.0f;
+        });
     }
 
     // The winner over the cluster; with top-p, unless the mass ahead of it is
     // below the limit, the race again among the classes ahead of it.
     u64 won;
     for (bool first_turn = true;; first_turn = false) {
-        const u64 mine = block_max64(sorted ? listed_best : race.best(wt), s);
+        const u64 mine = block_max64(by_list ? best : race.best(wt), s);
         const unsigned slot = turn++ & 1;
         tell_all(cluster, s, [&](Shared& o) { o.best[slot][rank] = mine; });
         row_sync(cluster);
         won = 0;
         for (unsigned r = 0; r < C; ++r) won = max(won, s.best[slot][r]);
-        if (!by_p || sorted || won == 0) break;
+        if (!by_p || won == 0) break;
         if (first_turn && !k) limit = static_cast<double>(p_in) * over_cluster(s.total);
         const unsigned i = ~static_cast<unsigned>(won);
         const Ahead ahead(key_of(x[i], i));
         double mass = 0.0;
-        each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
-            if (__any_sync(0xffffffffu, largest(v) >= ahead.x)) mass += sum4(ahead.only(v, j, wt.quick(v)));
-        });
+        if (by_list) {  // what is ahead of it reaches min-p too
+            for (unsigned c = t; c < s.listed; c += THREADS) {
+                const float u = key_logit(list[c]);
+                // whole multiples of 2^-40: the same sum in any order
+                if (ahead.of(u, key_index(list[c]))) mass += static_cast<double>(__float2ull_rn(wt.quick(u) * 0x1p40f)) * 0x1p-40;
+            }
+        } else {
+            each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
+                if (__any_sync(0xffffffffu, largest(v) >= ahead.x)) mass += sum4(ahead.only(v, j, wt.quick(v)));
+            });
+        }
         if (mass_of_all(mass, slot) < limit) break;
-        race.restart();
-        race_those([&](const float4& v, unsigned j, float4& w) { w = ahead.only(v, j, w); });
+        if (by_list) {
+            race_listed([&](float u, unsigned j) { return ahead.of(u, j); });
+        } else {
+            race.restart();
+            race_those([&](const float4& v, unsigned j, float4& w) { w = ahead.only(v, j, w); });
+        }
     }
-    if (rank == 0 && t == 0) {
-        const unsigned token = won == 0 ? key_index(top) : ~static_cast<unsigned>(won);
-        a.token[row] = token;
-        a.logprob[row] = wt.distance(x[token]) - logf(static_cast<float>(over_cluster(s.total)));
-    }
-    cluster.sync();  // nobody leaves while its shared memory may be written
+    answer(won);
 }
 
 template <unsigned THREADS>
