@@ -58,7 +58,7 @@ template <unsigned THREADS>
 constexpr unsigned kList = THREADS < 512 ? 2048 : 4096;  // classes a CTA lists
 constexpr unsigned kSorted = 512;      // classes that are sorted, of the whole cluster
 constexpr unsigned kGroups = 512;      // of threads, over the cluster, whose maxima bound the top k
-constexpr unsigned kMaxWarps = 32;
+constexpr unsigned kMaxWarps = 16;
 constexpr unsigned kIndexBits = 23;    // a key is 32 ordered logit bits, then these of ~index
 constexpr std::size_t kMaxVocab = 1u << kIndexBits;
 constexpr unsigned kKeyBits = 32 + kIndexBits;
@@ -685,7 +685,7 @@ sample_kernel(const SampleArgs a) {
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
     // the maxima of groups of neighbouring threads, 2k groups if there are as many
     const bool few = k && k <= kSorted / 2;
-    const unsigned warps = C * THREADS / 32;  // of the cluster, at most 256
+    const unsigned warps = C * THREADS / 32;  // of the cluster, at most 128
     const unsigned per_warp = groups_a_warp(warps, k), groups = warps * per_warp;
     if (few) {
         const unsigned lanes = 32 / per_warp;
@@ -865,6 +865,7 @@ sample_kernel(const SampleArgs a) {
         if (!by_p || won == 0) break;
         if (first_turn && !k) limit = static_cast<double>(p_in) * over_cluster(s.total);
         const unsigned i = ~static_cast<unsigned>(won);
+        if (i == key_index(top)) break;  // nothing is ahead of it
         const Ahead ahead(key_of(x[i], i));
         double mass = 0.0;
         if (by_list) {  // what is ahead of it reaches min-p too
@@ -907,29 +908,29 @@ void launch_rows(const SampleArgs& a, unsigned rows, unsigned C) {
 
 // Up to here four CTAs of 256 threads an SM are faster than two of 512: a row is
 // mostly barriers (512 rows of 4000 classes: 22 us against 28; 256 of 128000,
-// the other way, 131 against 140).
+// the other way, 98 against 105).
 constexpr bool vocab_fits_four(unsigned vocab) { return vocab <= 16384; }
 
 // Few rows are bound by the latency of their passes and barriers: as many CTAs a
-// row as leave each an SM of its own and 3200 classes, of 512 threads up to 16384
-// classes and of 1024 beyond (1 x 32000: 8.9 us with 512, 10.6 with 1024; 48 x
-// 50257 the other way, 29 and 27). With more rows, two CTAs of 512 threads an SM,
-// so that one's passes run through the other's barriers, and as many of them a
-// row (which is read more than once where there are filters) as keep the rows
-// that run together within 48 MB: beyond that L2 loses a row between its passes
-// (160 x 200000: 110 us, with half as many CTAs a row 126).
+// row, of 512 threads, as leave each an SM of its own and 1600 classes (16 x 8000:
+// 11.6 us, with 3200 classes 12.8), or half an SM and 4800 (64 x 128000: 45 us
+// against 50 alone on an SM; 140 x 8000 the other way, 21 against 18). With more
+// rows, two CTAs an SM, so that one's passes run through the other's barriers, and
+// as many of them a row (which is read more than once where there are filters) as
+// keep the rows that run together within 48 MB: beyond that L2 loses a row between
+// its passes (256 x 128000: 98 us, with half as many CTAs a row 106).
 void launch_sample(SampleArgs& a, std::size_t rows) {
     const u64 sms = static_cast<unsigned>(sm_count());
     const bool filtered = a.top_k || a.top_p || a.min_p;
     unsigned C = 1;
-    while (C < kMaxCluster && ((2 * rows * C <= sms && a.vocab / (2 * C) >= 3200) ||
-                               (filtered && rows > sms && 2 * sms / C * a.vocab * sizeof(float) > 48ull << 20)))
+    while (C < kMaxCluster &&
+           ((2 * rows * C <= sms && a.vocab / (2 * C) >= 1600) || (rows * C <= sms && a.vocab / (2 * C) >= 4800) ||
+            (filtered && rows * C > sms && 2 * sms / C * a.vocab * sizeof(float) > 48ull << 20)))
         C *= 2;
     a.chunk = ((a.vocab + C - 1) / C + 3) / 4 * 4;
     if (rows * C > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "sample: too many rows");
     const unsigned n = static_cast<unsigned>(rows);
-    if (rows * C <= sms && a.chunk > 16384) launch_rows<1024>(a, n, C);
-    else if (rows * C <= sms || !vocab_fits_four(a.vocab)) launch_rows<512>(a, n, C);
+    if (rows * C <= sms || !vocab_fits_four(a.vocab)) launch_rows<512>(a, n, C);
     else launch_rows<256>(a, n, C);
 }
 
