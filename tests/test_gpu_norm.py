@@ -168,6 +168,27 @@ def test_long_sums_over_rows(backend, rows, cols):
     within(backend.download(dw), edw, bdw, "dw")
 
 
+@pytest.mark.parametrize("rows,cols", [(7105, 1), (7107, 131), (7111, 33), (3600, 1000), (1801, 1030), (900, 2051),
+                                       (893, 4093), (449, 4099), (450, 8189), (450, 8191), (1000, 8192)])
+@pytest.mark.parametrize("shifted,over", [((), None), ((), "h"), (("dh",), None), (("gh", "w"), "gy"), ((), "gh")])
+def test_gradient_of_many_odd_rows(backend, rows, cols, shifted, over):
+    """Rows, or tensors beside h and gy, that start off the 16-byte grid."""
+    rng, x, _, w = inputs(rows, cols, 4)
+    host = {"h": x, "w": w, **{n: rng.normal(size=(rows, cols)).astype(np.float32) for n in ("gy", "gh")}}
+    host["dh"] = np.zeros((rows, cols), np.float32)
+    on, at = {}, {}
+    for name, v in host.items():
+        off = int(name in shifted)
+        on[name] = backend.upload(np.concatenate([np.zeros(off, np.float32), v.ravel()]))
+        at[name] = B.CudaStorage.borrow(on[name].ptr + 4 * off, v.size)
+    _, _, rstd = backend.rms_norm(at["h"], backend.upload(w), rows, cols)
+    dw, to = backend.allocate(cols), over or "dh"
+    backend.rms_norm_backward(at["h"], at["w"], rstd, at["gy"], rows, cols, gh=at["gh"], out=(at[to], dw))
+    edh, edw, bdh, bdw = R.rms_norm_backward(x, w, 1e-6, host["gy"], host["gh"])
+    within(backend.download(on[to])[int(to in shifted):].reshape(rows, cols), edh, bdh, "dh")
+    within(backend.download(dw), edw, bdw, "dw")
+
+
 def test_no_rows_and_repeatable(backend):
     w = backend.upload(np.ones(40, np.float32))
     empty = backend.allocate(0)

@@ -536,17 +536,25 @@ void launch_dw_finish(const float* partial, unsigned long long count, unsigned c
 // owns the same columns in every row, so dw adds up in its registers; the
 // groups' dw meet in shared memory and leave as one partial row a CTA, and the
 // partial rows are added in double.
+//
+// Rows whose length is no multiple of four start off the 16-byte grid, every
+// second or fourth of them alike: a CTA takes rows of one such class (`classes`
+// apart), copies each from the grid to the grid, and its threads' columns are
+// still the same in every row. (Columns by single floats instead took twice the
+// time.)
 constexpr unsigned kRingThreads = 512;
 constexpr unsigned kRingWarps = kRingThreads / 32;
 constexpr unsigned kRingCols = 8192;  // three stages of two rows fit an SM
-constexpr unsigned kRingSmem = 3 * 2 * kRingCols * sizeof(float);
+constexpr unsigned kRingSmem = 3 * 2 * (kRingCols + 4) * sizeof(float);
 constexpr unsigned kRingMaxStages = 8;
 
 struct RingArgs {
     NormBwdArgs n;
     unsigned T, R;          // threads a row, rows a block
     unsigned stages;
-    unsigned long long blocks;
+    unsigned classes;       // 1, 2 or 4; the grid is a multiple of it
+    unsigned pitch;         // floats between rows in a stage
+    unsigned long long blocks;  // of the largest class
     unsigned segments;      // of kDwRows blocks, the CTA with the most
     float* partial;         // [grid][segments - 1][R][cols], then [grid][cols]
     unsigned* err;
@@ -559,61 +567,125 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned b
                  : "memory");
 }
 
-template <int NV>
-__global__ void __launch_bounds__(kRingThreads + 32, 1)
+template <bool SKEWED, int NV>
+__global__ void __launch_bounds__(kRingThreads + (SKEWED ? 64 : 32), 1)
 norm_bwd_ring(const RingArgs a) {
     extern __shared__ __align__(128) float ring[];
-    __shared__ unsigned long long full[kRingMaxStages], empty[kRingMaxStages];
+    __shared__ unsigned long long full[kRingMaxStages], empty[kRingMaxStages], clean[SKEWED ? kRingMaxStages : 1];
     __shared__ double slots[3][kRingWarps];
     __shared__ unsigned dead_flag;
     volatile unsigned* dead = &dead_flag;
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned cols = a.n.cols, block_floats = a.R * cols;
+    const unsigned cols = a.n.cols, block_floats = a.R * a.pitch;
     const unsigned stage_floats = 2 * block_floats;
+    // this CTA's class and its rows' skew, its first block and the step to the next
+    const unsigned classes = SKEWED ? a.classes : 1, kind = SKEWED ? blockIdx.x % classes : 0;
+    const Span span{SKEWED ? (kind * cols) & 3 : 0, cols};
+    const unsigned long long begin = blockIdx.x / classes;
+    const unsigned step = gridDim.x / classes;
+    const auto row_at = [&](unsigned long long b, unsigned r) { return (b * a.R + r) * classes + kind; };
     if (threadIdx.x == 0) {
         dead_flag = 0;
         for (unsigned s = 0; s < a.stages; ++s) {
             mbar_init(full + s, 1);
-            mbar_init(empty + s, kRingWarps);
+            if (SKEWED) mbar_init(clean + s, 1);
+            mbar_init(empty + s, a.R * a.T / 32);
         }
         mbar_fence_init();
     }
     __syncthreads();
 
     if (warp == kRingWarps) {  // producer
-        if (lane == 0) {
-            unsigned issued = 0;
-            for (unsigned long long b = blockIdx.x; b < a.blocks; b += gridDim.x, ++issued) {
-                const unsigned slot = issued % a.stages, turn = issued / a.stages;
-                if (turn && (*dead || !mbar_wait_bounded(empty + slot, (turn - 1) & 1, a.err, kWaitPolls / 8))) {
-                    *dead = 1;
-                    break;
-                }
+        unsigned issued = 0;
+        for (unsigned long long b = begin; b < a.blocks; b += step, ++issued) {
+            const unsigned slot = issued % a.stages, turn = issued / a.stages;
+            bool go = true;
+            if (turn && lane == 0)
+                go = !*dead && mbar_wait_bounded(empty + slot, (turn - 1) & 1, a.err, kWaitPolls / 8);
+            if (!__shfl_sync(0xffffffffu, go, 0)) {
+                *dead = 1;
+                break;
+            }
+            float* at = ring + slot * stage_floats;
+            if constexpr (!SKEWED) {
                 const unsigned long long row = b * a.R;
                 const unsigned rows = static_cast<unsigned>(min(static_cast<unsigned long long>(a.R), a.n.rows - row));
                 const unsigned bytes = rows * cols * sizeof(float);
-                float* at = ring + slot * stage_floats;
-                mbar_expect_tx(full + slot, 2 * bytes);
-                bulk_copy(at, a.n.h + row * cols, bytes, full + slot);
-                bulk_copy(at + block_floats, a.n.gy + row * cols, bytes, full + slot);
+                if (lane == 0) {
+                    mbar_expect_tx(full + slot, 2 * bytes);
+                    bulk_copy(at, a.n.h + row * cols, bytes, full + slot);
+                    bulk_copy(at + block_floats, a.n.gy + row * cols, bytes, full + slot);
+                }
+            } else {  // a row a lane
+                const unsigned long long row = row_at(b, lane), first = row * cols;
+                const bool have = lane < a.R && row < a.n.rows;
+                unsigned floats = have ? 4 * span.groups() : 0;
+                float* to = at + lane * a.pitch;
+                if (have && row + 1 == a.n.rows) {  // the tensors end with the row
+                    floats = (span.skew + cols) & ~3u;
+                    for (unsigned i = floats; i < span.skew + cols; ++i) {
+                        to[i] = a.n.h[first + i - span.skew];
+                        to[block_floats + i] = a.n.gy[first + i - span.skew];
+                    }
+                }
+                const unsigned all = __reduce_add_sync(0xffffffffu, floats);
+                if (lane == 0) mbar_expect_tx(full + slot, 2 * all * sizeof(float));
+                __syncwarp();
+                if (have) {
+                    bulk_copy(to, a.n.h + (first - span.skew), floats * sizeof(float), full + slot);
+                    bulk_copy(to + block_floats, a.n.gy + (first - span.skew), floats * sizeof(float), full + slot);
+                }
             }
-            // the copies still in flight land before the CTA may finish
+        }
+        // the copies still in flight land before the CTA may finish
+        if (lane == 0)
             for (unsigned s = issued > a.stages ? issued - a.stages : 0; s < issued; ++s)
                 mbar_wait_bounded(full + s % a.stages, (s / a.stages) & 1, a.err, kWaitPolls / 16);
+    } else if (SKEWED && warp > kRingWarps) {
+        // Zeros in the place of the neighbours' columns, a row a lane: the others
+        // then need no look at where a row begins and ends.
+        unsigned i_th = 0;
+        for (unsigned long long b = begin; b < a.blocks; b += step, ++i_th) {
+            const unsigned slot = i_th % a.stages;
+            bool go = true;
+            if (lane == 0) go = !*dead && mbar_wait_bounded(full + slot, (i_th / a.stages) & 1, a.err, kWaitPolls / 8);
+            if (!__shfl_sync(0xffffffffu, go, 0)) {
+                *dead = 1;
+                break;
+            }
+            if (lane < a.R && row_at(b, lane) < a.n.rows) {
+                float* row = ring + slot * stage_floats + lane * a.pitch;
+                for (unsigned e = 0; e < span.skew; ++e) row[e] = row[block_floats + e] = 0.0f;
+                for (unsigned e = span.skew + cols; e < 4 * span.groups(); ++e) row[e] = row[block_floats + e] = 0.0f;
+            }
+            fence_proxy_async_smem();  // before the slot's next copy
+            __syncwarp();
+            if (lane == 0) mbar_arrive(clean + slot);
         }
     } else {
         const unsigned group = threadIdx.x / a.T, t = threadIdx.x - group * a.T;
-        const unsigned G = cols / 4;
+        const unsigned G = span.groups();
         // the weight stays in registers: the ring leaves L1 too little to hold it
         Group dw[NV], w[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             dw[i] = Group{};
-            w[i] = t + i * a.T < G ? load_weight<false>(a.n.w, t + i * a.T, Span{0, cols}) : Group{};
+            w[i] = t + i * a.T < G ? load_weight<SKEWED>(a.n.w, t + i * a.T, span) : Group{};
         }
+        // A thread's columns of a partial row, whose own rows are off the grid too.
+        const auto put = [&](float* out, unsigned at_c, const Group& v) {
+            if (at_c >= G) return;
+            if constexpr (!SKEWED) {
+                reinterpret_cast<float4*>(out)[at_c] = make_float4(v.v[0], v.v[1], v.v[2], v.v[3]);
+            } else {
+#pragma unroll
+                for (unsigned e = 0; e < 4; ++e)
+                    if (span.has(at_c, e)) out[4 * at_c + e - span.skew] = v.v[e];
+            }
+        };
         unsigned segment = 0;
         const double by_cols = 1.0 / cols;
-        const auto row_of = [&](unsigned long long b) { return b * a.R + group; };
+        const auto row_of = [&](unsigned long long b) { return row_at(b, group); };
         Group up[NV];  // gh of the row whose dot product was added up last
         float s_of = 0.0f;  // and its rstd
         // The dot product of block b's row, the i-th of this CTA; dw.
@@ -625,17 +697,21 @@ norm_bwd_ring(const RingArgs a) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const unsigned c = t + i * a.T;
-                up[i] = mine && a.n.gh && c < G ? load_group<false>(a.n.gh + row * cols, c, Span{0, cols}) : Group{};
+                up[i] = Group{};
+                if (mine && a.n.gh && c < G) {
+                    const float* gh = a.n.gh + row * cols;
+                    if (SKEWED && row + 1 == a.n.rows) up[i] = load_group<SKEWED>(gh, c, span);
+                    else up[i] = group_of(reinterpret_cast<const float4*>(gh - span.skew)[c]);
+                }
             }
-            if (!*dead && !mbar_wait_bounded(full + slot, (i_th / a.stages) & 1, a.err, kWaitPolls / 8)) *dead = 1;
-            const float* at = ring + slot * stage_floats + group * cols;
+            if (!*dead && !mbar_wait_bounded((SKEWED ? clean : full) + slot, (i_th / a.stages) & 1, a.err, kWaitPolls / 8)) *dead = 1;
+            const float* at = ring + slot * stage_floats + group * a.pitch;
             double dot = 0.0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const unsigned c = t + i * a.T;
                 if (mine && c < G) {
-                    const Group h = group_of(reinterpret_cast<const float4*>(at)[c]);
-                    const Group g = group_of(reinterpret_cast<const float4*>(at + block_floats)[c]);
+                    const Group h = group_of(reinterpret_cast<const float4*>(at)[c]), g = group_of(reinterpret_cast<const float4*>(at + block_floats)[c]);
                     float part = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -655,26 +731,29 @@ norm_bwd_ring(const RingArgs a) {
             const double dot = warp_sum(lane < a.T >> 5 ? slots[i_th % 3][group * (a.T >> 5) + lane] : 0.0);
             const float c = static_cast<float>(dot * by_cols) * (s * s);
             if (row < a.n.rows) {
-                const float* at = ring + slot * stage_floats + group * cols;
-                float4* dh = reinterpret_cast<float4*>(a.n.dh + row * cols);
+                const float* at = ring + slot * stage_floats + group * a.pitch;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     const unsigned at_c = t + i * a.T;
                     if (at_c >= G) continue;
-                    const Group h = group_of(reinterpret_cast<const float4*>(at)[at_c]);
-                    const Group g = group_of(reinterpret_cast<const float4*>(at + block_floats)[at_c]);
-                    float o[4];
+                    const Group h = group_of(reinterpret_cast<const float4*>(at)[at_c]), g = group_of(reinterpret_cast<const float4*>(at + block_floats)[at_c]);
+                    Group o;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = fmaf(s, fmaf(-h.v[e], c, g.v[e] * w[i].v[e]), gh[i].v[e]);
-                    __stcs(dh + at_c, make_float4(o[0], o[1], o[2], o[3]));
+                    for (int e = 0; e < 4; ++e) o.v[e] = fmaf(s, fmaf(-h.v[e], c, g.v[e] * w[i].v[e]), gh[i].v[e]);
+                    float* dh = a.n.dh + row * cols;
+                    if (!SKEWED || (at_c > 0 && at_c < G - 1))
+                        __stcs(reinterpret_cast<float4*>(dh - span.skew) + at_c, make_float4(o.v[0], o.v[1], o.v[2], o.v[3]));
+                    else
+                        put(dh, at_c, o);
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(empty + slot);
         };
         unsigned used = 0;
-        if (blockIdx.x < a.blocks) take(blockIdx.x, 0);
-        for (unsigned long long b = blockIdx.x; b < a.blocks; b += gridDim.x, ++used) {
+        const bool works = !SKEWED || group < a.R;  // some threads may be over
+        if (works && begin < a.blocks) take(begin, 0);
+        for (unsigned long long b = begin; works && b < a.blocks; b += step, ++used) {
             Group gh[NV];
 #pragma unroll
             for (int i = 0; i < NV; ++i) gh[i] = up[i];
@@ -683,75 +762,77 @@ norm_bwd_ring(const RingArgs a) {
                 float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const unsigned at_c = t + i * a.T;
-                    if (at_c < G)
-                        reinterpret_cast<float4*>(out)[at_c] = make_float4(dw[i].v[0], dw[i].v[1], dw[i].v[2], dw[i].v[3]);
+                    put(out, t + i * a.T, dw[i]);
                     dw[i] = Group{};
                 }
                 ++segment;
             }
-            if (b + gridDim.x < a.blocks) take(b + gridDim.x, used + 1);
+            if (b + step < a.blocks) take(b + step, used + 1);
             if (a.T > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(a.T) : "memory");
             else __syncwarp();
             give(b, used, gh, s);
         }
-        for (; segment + 1 < a.segments; ++segment) {  // CTAs with fewer blocks
+        for (; works && segment + 1 < a.segments; ++segment) {  // CTAs with fewer blocks
             float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if (t + i * a.T < G) reinterpret_cast<float4*>(out)[t + i * a.T] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int i = 0; i < NV; ++i) put(out, t + i * a.T, Group{});
         }
         // the groups' rows meet in the ring, which nothing reads any more
         asm volatile("bar.sync 15, %0;" ::"n"(kRingThreads) : "memory");
-        float4* rows = reinterpret_cast<float4*>(ring);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (t + i * a.T < G)
-                rows[group * G + t + i * a.T] = make_float4(dw[i].v[0], dw[i].v[1], dw[i].v[2], dw[i].v[3]);
+            if (works) put(ring + group * cols, t + i * a.T, dw[i]);
         asm volatile("bar.sync 15, %0;" ::"n"(kRingThreads) : "memory");
-        float4* out = reinterpret_cast<float4*>(a.partial + (static_cast<unsigned long long>(gridDim.x) * (a.segments - 1) * a.R + blockIdx.x) * cols);
-        for (unsigned c = threadIdx.x; c < G; c += kRingThreads) {
-            float4 sum = rows[c];
-            for (unsigned r = 1; r < a.R; ++r) {
-                const float4 v = rows[r * G + c];
-                sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-            }
+        float* out = a.partial + (static_cast<unsigned long long>(gridDim.x) * (a.segments - 1) * a.R + blockIdx.x) * cols;
+        for (unsigned c = threadIdx.x; c < cols; c += kRingThreads) {
+            float sum = ring[c];
+            for (unsigned r = 1; r < a.R; ++r) sum += ring[r * cols + c];
             out[c] = sum;
         }
     }
 }
 
-template <int NV>
-void launch_ring(const RingArgs& a, unsigned ctas, unsigned smem) {
-    allow_smem<norm_bwd_ring<NV>, kRingSmem>();
-    norm_bwd_ring<NV><<<ctas, kRingThreads + 32, smem, stream()>>>(a);
+template <bool SKEWED, int NV>
+void launch_ring_nv(const RingArgs& a, unsigned ctas, unsigned smem) {
+    allow_smem<norm_bwd_ring<SKEWED, NV>, kRingSmem>();
+    norm_bwd_ring<SKEWED, NV><<<ctas, kRingThreads + (SKEWED ? 64 : 32), smem, stream()>>>(a);
+}
+template <bool SKEWED>
+void launch_ring(const RingArgs& a, unsigned groups, unsigned ctas, unsigned smem) {
+    const unsigned per = (groups + a.T - 1) / a.T;
+    if (per <= 1) launch_ring_nv<SKEWED, 1>(a, ctas, smem);
+    else if (per <= 2) launch_ring_nv<SKEWED, 2>(a, ctas, smem);
+    else launch_ring_nv<SKEWED, 4>(a, ctas, smem);
 }
 
 // The fused pass, where it applies; false, having launched nothing, otherwise.
 bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
-    if (n.cols % 4 != 0 || n.cols > kRingCols || !aligned16(n.h) || !aligned16(n.gy) || !aligned16(n.w) ||
-        !aligned16(n.dh) || (n.gh && !aligned16(n.gh)))
-        return false;
+    if (!aligned16(n.h) || !aligned16(n.gy) || !aligned16(n.dh) || (n.gh && !aligned16(n.gh))) return false;
+    const bool skewed = n.cols % 4 != 0 || !aligned16(n.w);
+    const unsigned groups = skewed ? (n.cols + 3 + 3) / 4 : n.cols / 4;  // at most
+    // (a row's copy may reach three floats into the next row)
+    if (groups > kRingCols / 4 || n.cols < 4) return false;
     RingArgs a{};
     a.n = n;
-    a.T = 32;
-    while (a.T < kRingThreads && a.T * 16 < n.cols) a.T *= 2;  // up to four groups a thread
-    a.R = kRingThreads / a.T;
-    a.blocks = (n.rows + a.R - 1) / a.R;
-    const unsigned sms = static_cast<unsigned>(sm_count());
-    if (a.blocks < 3ull * sms) return false;
-    const unsigned stage = 2 * a.R * n.cols * sizeof(float);
+    // up to four groups a thread; rows of 2^n floats and their neighbours off the
+    // grid need one group more, and 3 or 5 rows a block instead of half of 4 or 8
+    for (a.R = 16; a.R > 1 && 4 * (kRingThreads / a.R / 32 * 32) < groups;) a.R = skewed ? a.R - 1 : a.R / 2;
+    a.T = kRingThreads / a.R / 32 * 32;
+    a.classes = n.cols % 4 == 0 ? 1 : n.cols % 2 == 0 ? 2 : 4;
+    a.pitch = skewed ? 4 * groups : n.cols;
+    const unsigned ctas = static_cast<unsigned>(sm_count()) / a.classes * a.classes, step = ctas / a.classes;
+    a.blocks = ((n.rows + a.classes - 1) / a.classes + a.R - 1) / a.R;
+    if (a.blocks < 3ull * step) return false;
+    const unsigned stage = 2 * a.R * a.pitch * sizeof(float);
     a.stages = std::min(kRingMaxStages, kRingSmem / stage);
-    const unsigned long long most = (a.blocks + sms - 1) / sms;
+    const unsigned long long most = (a.blocks + step - 1) / step;
     a.segments = static_cast<unsigned>((most + kDwRows - 1) / kDwRows);
-    const unsigned long long partial_rows = static_cast<unsigned long long>(sms) * ((a.segments - 1) * a.R + 1);
+    const unsigned long long partial_rows = static_cast<unsigned long long>(ctas) * ((a.segments - 1) * a.R + 1);
     Scratch partial(partial_rows * n.cols * sizeof(float));
     a.partial = partial.as<float>();
     a.err = device_error_word();
-    const unsigned per = (n.cols / 4 + a.T - 1) / a.T;
-    if (per <= 1) launch_ring<1>(a, sms, a.stages * stage);
-    else if (per <= 2) launch_ring<2>(a, sms, a.stages * stage);
-    else launch_ring<4>(a, sms, a.stages * stage);
+    if (skewed) launch_ring<true>(a, groups, ctas, a.stages * stage);
+    else launch_ring<false>(a, groups, ctas, a.stages * stage);
     check_launch("norm_bwd_ring");
     launch_dw_finish(a.partial, partial_rows, n.cols, dw);
     return true;
