@@ -525,23 +525,26 @@ void launch_dw_finish(const float* partial, unsigned long long count, unsigned c
     check_launch("norm_dw_finish");
 }
 
-// dh and dw from one pass over h, gy and gh, for aligned rows of up to
-// kRingCols floats: 16 B an element is all that moves. One CTA an SM walks
-// blocks of R rows (R groups of T threads, T * R = kRingThreads). A producer
-// warp bulk-copies the blocks of h and gy into a ring of shared-memory stages;
-// gh is loaded a block ahead into registers. A group adds up the dot product of
-// its next row before it writes dh of its current one, so that the one barrier a
-// row and the sums' latency lie behind work that does not depend on them (the
-// same ring without that, a row at a time: 232 us for 8192 x 8192). A thread
-// owns the same columns in every row, so dw adds up in its registers; the
-// groups' dw meet in shared memory and leave as one partial row a CTA, and the
-// partial rows are added in double.
+// dh and dw from one pass over h, gy and gh, for rows of up to kRingCols floats:
+// 16 B an element is all that moves. One CTA an SM walks blocks of R rows (R
+// groups of T threads). A producer warp bulk-copies the blocks of h and gy into a
+// ring of shared-memory stages; gh is loaded a block ahead into registers. A group
+// adds up the dot product of its next row before it writes dh of its current one,
+// so that the one barrier a row and the sums' latency lie behind work that does
+// not depend on them (8192 x 8192 a row at a time: 232 us, so: 189). A thread owns
+// the same columns in every row, so dw adds up in its registers; the groups' dw
+// meet in shared memory and leave as one partial row a CTA, and the partial rows
+// are added in double.
 //
 // Rows whose length is no multiple of four start off the 16-byte grid, every
 // second or fourth of them alike: a CTA takes rows of one such class (`classes`
 // apart), copies each from the grid to the grid, and its threads' columns are
-// still the same in every row. (Columns by single floats instead took twice the
-// time.)
+// still the same in every row. A warp of its own zeroes the neighbours' columns
+// that come with a copy (with every thread looking for them 30000 x 2047 took 347
+// us, now 253; with columns by single floats 458, with dh and dw by themselves 327).
+//
+// HBM bounds the even lengths (8192 x 8192: 5.67 TB/s, 30000 x 2048 in 161 us: 6.1
+// TB/s), instructions the odd ones, those at the rows' ends above all.
 constexpr unsigned kRingThreads = 512;
 constexpr unsigned kRingWarps = kRingThreads / 32;
 constexpr unsigned kRingCols = 8192;  // three stages of two rows fit an SM

@@ -153,11 +153,13 @@ struct Shared {
     u64 warp64[kMaxWarps];
     double warpd[kMaxWarps];
     unsigned listed, picked;
+    unsigned first;  // class that has the row's maximum, of this CTA's (~0: none)
     unsigned found_bin, found_in;  // kBins: none
     u64 found_ahead;
     // written by every CTA of the cluster, by its rank
     u64 top[kMaxCluster], best[2][kMaxCluster];
     double total[kMaxCluster], mass[2][kMaxCluster];
+    unsigned firsts[kMaxCluster];
     u64 share[kMaxCluster];
 };
 
@@ -593,8 +595,8 @@ template <unsigned THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS)
 sample_kernel(const SampleArgs a) {
     __shared__ Shared s;
-    // the keys of the classes that may be left; later the sorted ones, with their numbers
-    __shared__ u64 list[kList<THREADS>];
+    // (logit, index) of the classes that may be left; later the sorted ones' keys, and their numbers
+    __shared__ uint2 list[kList<THREADS>];
     const cg::cluster_group cluster = cg::this_cluster();
     const unsigned C = cluster.num_blocks(), rank = cluster.block_rank();
     const u64 row = blockIdx.x / C;
@@ -673,15 +675,14 @@ sample_kernel(const SampleArgs a) {
             if (!first_only) race.template run<THREADS>(wt, w, e, first);
         });
     } else {
-        each_batch<THREADS, 4>(x, begin, end, [&](const auto& v, unsigned i, auto loose) {
-            own_peak = fmaxf(own_peak, largest(v));
-            peak.template see<THREADS>(v, i, loose);
-        });
+        each_batch<THREADS, 4>(x, begin, end,
+                               [&](const auto& v, unsigned, auto) { own_peak = fmaxf(own_peak, largest(v)); });
     }
-    u64 top = 0;
+    u64 top = 0;  // (whose index the next pass finds where there is one)
+    if (!at_once && in_play(own_peak)) top = key_of(own_peak, 0);
     if (peak.at != 0xffffffffu) top = key_of(peak.high < kLargest ? peak.high : x[peak.at], peak.at);
     top = block_max64(top, s);
-    if (t == 0) s.listed = s.picked = 0;
+    if (t == 0) s.listed = s.picked = 0, s.first = 0xffffffffu;
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
     // the maxima of groups of neighbouring threads, 2k groups if there are as many
     const bool few = k && k <= kSorted / 2;
@@ -704,7 +705,7 @@ sample_kernel(const SampleArgs a) {
         }
         return;
     }
-    const float high = capped(key_logit(top));
+    const float most = key_logit(top), high = capped(most);
     if (at_once) total *= exp2_quick((wt.m - high) * wt.to_log2);
     wt.m = high;
 
@@ -714,11 +715,36 @@ sample_kernel(const SampleArgs a) {
     float cut = -INFINITY;
     if (few && k <= groups) cut = kth_of<THREADS>(s, s.group, groups, static_cast<unsigned>(k));
     const bool picking = in_play(cut), listing = min_p > 0.0f && !k;
-    if (picking) {
+    const auto find_first = [&](const float4& v, unsigned i) {
+        const unsigned at = v.x == most ? i : v.y == most ? i + 1 : v.z == most ? i + 2 : v.w == most ? i + 3 : 0xffffffffu;
+        if (at != 0xffffffffu) atomicMin(&s.first, at);
+    };
+    if (listing) {
+        bool full = false;
+        const float least = min_p * (1.0f - kNear);  // the rest of the decision is the race's
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+            const float4 w = wt.quick(v);
+            total += sum4(w);
+            if (!(largest(w) >= least)) return;
+            find_first(v, i);
+            const bool x1 = w.x >= least, y1 = w.y >= least, z1 = w.z >= least, w1 = w.w >= least;
+            const unsigned n = x1 + y1 + z1 + w1;
+            unsigned at = full ? kList<THREADS> : atomicAdd(&s.listed, n);
+            full = at + n > kList<THREADS>;
+            if (full) return;
+            if (x1) list[at++] = make_uint2(__float_as_uint(v.x), i);
+            if (y1) list[at++] = make_uint2(__float_as_uint(v.y), i + 1);
+            if (z1) list[at++] = make_uint2(__float_as_uint(v.z), i + 2);
+            if (w1) list[at] = make_uint2(__float_as_uint(v.w), i + 3);
+        });
+    } else if (!at_once) {
         Shared* one = cluster.map_shared_rank(&s, 0);
+        const float from = picking ? cut : most;
         each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
             total += sum4(wt.quick(v));
-            if (!(largest(v) >= cut)) return;
+            if (!(largest(v) >= from)) return;
+            find_first(v, i);
+            if (!picking) return;
             const auto picks = [&](float u, unsigned j) {
                 if (u >= cut && in_play(u)) {
                     const unsigned at = atomicAdd(&one->picked, 1u);
@@ -727,32 +753,25 @@ sample_kernel(const SampleArgs a) {
             };
             picks(v.x, i), picks(v.y, i + 1), picks(v.z, i + 2), picks(v.w, i + 3);
         });
-    } else if (!at_once) {
-        float least = listing ? min_p * (1.0f - kNear) : INFINITY;
-        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
-            const float4 w = wt.quick(v);
-            total += sum4(w);
-            if (!(largest(w) >= least)) return;
-            const auto lists = [&](float u, float w, unsigned j) {
-                if (w >= least && wt.reaches(min_p, w, u)) {
-                    const unsigned at = atomicAdd(&s.listed, 1u);
-                    if (at < kList<THREADS>) list[at] = key_of(u, j);
-                    else least = INFINITY;  // the list is full
-                }
-            };
-            lists(v.x, w.x, i), lists(v.y, w.y, i + 1), lists(v.z, w.z, i + 2), lists(v.w, w.w, i + 3);
-        });
     }
     total = block_sum_d(total, s);
-    tell_all(cluster, s, [&](Shared& o) { o.total[rank] = total; });
+    tell_all(cluster, s, [&](Shared& o) {
+        o.total[rank] = total;
+        o.firsts[rank] = s.first;
+    });
     const auto over_cluster = [&](const double* parts) {
         double all = 0.0;
         for (unsigned r = 0; r < C; ++r) all += parts[r];
         return all;
     };
+    const auto first_class = [&] {
+        unsigned i = at_once ? key_index(top) : s.firsts[0];
+        for (unsigned r = 1; r < C && !at_once; ++r) i = min(i, s.firsts[r]);
+        return i;
+    };
     const auto answer = [&](u64 won) {
         if (rank != 0 || t != 0) return;
-        const unsigned token = won == 0 ? key_index(top) : ~static_cast<unsigned>(won);
+        const unsigned token = won == 0 ? first_class() : ~static_cast<unsigned>(won);
         a.token[row] = token;
         a.logprob[row] = wt.distance(x[token]) - logf(static_cast<float>(over_cluster(s.total)));
     };
@@ -764,14 +783,15 @@ sample_kernel(const SampleArgs a) {
             if (rank != 0) return;
             // the classes in order, `per` a thread: the filters, then the race of the ones left
             constexpr unsigned per = kSorted > THREADS ? kSorted / THREADS : 1;
+            u64* sorted = reinterpret_cast<u64*>(list);
             float* numbers = reinterpret_cast<float*>(list + kSorted);
-            sort_picks<THREADS>(s, picked, race.noise, list, numbers);
+            sort_picks<THREADS>(s, picked, race.noise, sorted, numbers);
             u64 key[per], mass[per], sum = 0, best = 0;
             float w[per];
 #pragma unroll
             for (unsigned j = 0; j < per; ++j) {
                 const unsigned at = t * per + j;
-                key[j] = at < picked && at < k ? list[at] : 0;
+                key[j] = at < picked && at < k ? sorted[at] : 0;
                 w[j] = key[j] ? wt.quick(key_logit(key[j])) : 0.0f;
                 mass[j] = __float2ull_rn(w[j] * 0x1p40f);  // whole numbers: exact sums in any order
                 sum += mass[j];
@@ -808,13 +828,13 @@ sample_kernel(const SampleArgs a) {
         best = 0;
 #pragma unroll
         for (unsigned j = 0; j < per; ++j)
-            if (t + j * THREADS < s.listed) e[j] = race.noise[key_index(list[t + j * THREADS])];
+            if (t + j * THREADS < s.listed) e[j] = race.noise[list[t + j * THREADS].y];
 #pragma unroll
         for (unsigned j = 0; j < per; ++j) {
             if (t + j * THREADS >= s.listed) break;
-            const u64 key = list[t + j * THREADS];
-            const float u = key_logit(key);
-            if (joins(u, key_index(key))) best = max(best, exact_score(u, e[j], key_index(key), wt.m, wt.t));
+            const uint2 c = list[t + j * THREADS];
+            const float u = __uint_as_float(c.x);
+            if (joins(u, c.y)) best = max(best, exact_score(u, e[j], c.y, wt.m, wt.t));
         }
     };
     double limit = 0.0;
@@ -825,7 +845,7 @@ sample_kernel(const SampleArgs a) {
             if (!(largest(v) >= key_logit(least))) return;
             const auto keep = [&](float u, unsigned j) {
                 if (!in_play(u) || key_of(u, j) < least) return 0.0f;
-                if (by_list) list[atomicAdd(&s.listed, 1u)] = key_of(u, j);
+                if (by_list) list[atomicAdd(&s.listed, 1u)] = make_uint2(__float_as_uint(u), j);
                 return wt.quick(u);
             };
             mass += sum4(make_float4(keep(v.x, i), keep(v.y, i + 1), keep(v.z, i + 2), keep(v.w, i + 3)));
@@ -842,7 +862,7 @@ sample_kernel(const SampleArgs a) {
             });
         }
     } else if (by_list) {
-        race_listed([](float, unsigned) { return true; });
+        race_listed([&](float u, unsigned) { return wt.reaches(min_p, wt.quick(u), u); });
     } else if (!at_once) {
         race_those([&](const float4& v, unsigned, float4& w) {
             if (!wt.reaches(min_p, w.x, v.x)) w.x = 0.0f;
@@ -865,14 +885,14 @@ sample_kernel(const SampleArgs a) {
         if (!by_p || won == 0) break;
         if (first_turn && !k) limit = static_cast<double>(p_in) * over_cluster(s.total);
         const unsigned i = ~static_cast<unsigned>(won);
-        if (i == key_index(top)) break;  // nothing is ahead of it
+        if (i == first_class()) break;  // nothing is ahead of it
         const Ahead ahead(key_of(x[i], i));
         double mass = 0.0;
         if (by_list) {  // what is ahead of it reaches min-p too
             for (unsigned c = t; c < s.listed; c += THREADS) {
-                const float u = key_logit(list[c]);
+                const float u = __uint_as_float(list[c].x);
                 // whole multiples of 2^-40: the same sum in any order
-                if (ahead.of(u, key_index(list[c]))) mass += static_cast<double>(__float2ull_rn(wt.quick(u) * 0x1p40f)) * 0x1p-40;
+                if (ahead.of(u, list[c].y)) mass += static_cast<double>(__float2ull_rn(wt.quick(u) * 0x1p40f)) * 0x1p-40;
             }
         } else {
             each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
