@@ -46,6 +46,12 @@ def test_product(backend, m, n, k):
         check(backend, a, b, k, sa, sb, bias, backend.download(out).reshape(m, n), f"{m}x{n}x{k} pitch {pitch}")
 
 
+@pytest.mark.parametrize("m,n,k", [(17, 18944, 40), (33, 18945, 130), (70, 20001, 300), (200, 19500, 64), (256, 38001, 16)])
+def test_wide_products_of_one_tile_of_tokens(backend, m, n, k):
+    """More weight rows than one tile a pair of CTAs: tiles have fewer than 128."""
+    test_product(backend, m, n, k)
+
+
 @pytest.mark.parametrize("m,n", [(1, 3), (9, 130), (70, 40), (300, 260)])
 def test_largest_sums(backend, m, n):
     """The longest rows of the largest values: 131071 * 2^14 < 2^31."""

@@ -152,6 +152,7 @@ struct TcArgs {
     float* out;
     unsigned m, n;
     unsigned bn;          // tokens a tile, a multiple of 16
+    unsigned rows;        // weight rows a CTA's tile, at most kTileM, a multiple of 8
     unsigned steps;       // along k: stages a tile takes
     unsigned tiles_m;     // along the tokens
     unsigned tiles_n;     // along the weights
@@ -248,13 +249,31 @@ __device__ __forceinline__ void tile_at(unsigned i, const TcArgs& g, unsigned& t
     tn = band * kGroup + in - tm * width;
 }
 
+// What a store thread needs beside the sums of its weight row, loaded while the
+// sums are on their way: they come from HBM, and fetched after them, with the other
+// CTAs' sums one after another, 256 x 4096 x 4096 took 15.8 us, so 13.0. The tokens'
+// scales are read later, from L1.
+struct RowScale {
+    bool mine;
+    float scale, bias;
+};
+__device__ __forceinline__ RowScale row_scale(const TcArgs& g, unsigned first, unsigned row0) {
+    const unsigned lane = threadIdx.x & 31, col = first + lane, token = row0 + 8 * lane;
+    RowScale r{col < g.n && (threadIdx.x >> 5 & 3) * 32 + lane < g.rows, 0.0f, 0.0f};
+    if (r.mine) r.scale = __ldg(g.sb + col);
+    if (r.mine && g.bias) r.bias = __ldg(g.bias + col);
+    float touched;  // 8 of them a sector, at most 256 a tile
+    if (token < g.m && 8 * lane < g.bn)
+        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(touched) : "l"(g.sa + token));
+    return r;
+}
+
 // A warp's share of a finished tile: 32 weight rows (TMEM lanes, `first` the
 // lowest) and every other 16 tokens, scaled and stored, 128 bytes of one token at
 // a time. The next 16 leave TMEM while the present ones are stored.
-__device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsigned first, unsigned row0) {
+__device__ __forceinline__ void store_tile(const TcArgs& g, const RowScale& r, unsigned tmem, unsigned first,
+                                           unsigned row0) {
     const unsigned warp = threadIdx.x >> 5, col = first + (threadIdx.x & 31);
-    const bool mine = col < g.n;
-    const float sb = mine ? g.sb[col] : 0.0f, bias = mine && g.bias ? g.bias[col] : 0.0f;
     const unsigned rows = min(g.bn, g.m - row0), step = 16 * (kStoreWarps / 4);
     const unsigned taddr = tmem + ((warp & 3) * 32 << 16);
     const float* sa = g.sa + row0;
@@ -278,17 +297,17 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
         __syncwarp();
         tmem_load_wait();
 #pragma unroll
-        for (unsigned j = 0; j < 16; ++j) s[j] = static_cast<float>(v[j]) * (s[j] * sb);
+        for (unsigned j = 0; j < 16; ++j) s[j] = static_cast<float>(v[j]) * (s[j] * r.scale);
         if (g.bias) {
 #pragma unroll
-            for (unsigned j = 0; j < 16; ++j) s[j] += bias;
+            for (unsigned j = 0; j < 16; ++j) s[j] += r.bias;
         }
         if (c + step < rows) tmem_load16(taddr + c + step, v);
         float* out = g.out + static_cast<unsigned long long>(row0 + c) * g.n + col;
-        if (mine && c + 16 <= rows) {
+        if (r.mine && c + 16 <= rows) {
 #pragma unroll
             for (unsigned j = 0; j < 16; ++j) out[static_cast<unsigned long long>(j) * g.n] = s[j];
-        } else if (mine) {
+        } else if (r.mine) {
 #pragma unroll
             for (unsigned j = 0; j < 16; ++j)
                 if (c + j < rows) out[static_cast<unsigned long long>(j) * g.n] = s[j];
@@ -304,6 +323,7 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, unsigned tmem, unsig
 // us on the exchange by way of shared memory, 16 in all without it). Clusters of
 // eight found fewer places on the GPU: 64 x 2048 x 4096 took 18 us with them, 10
 // with four. One tile a CTA, no double buffer.
+constexpr unsigned kMostSplit = 4;
 struct SplitArgs {
     TcArgs g;
     unsigned split;       // CTAs a tile, 1, 2 or 4
@@ -361,6 +381,7 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = tmem_base;
+    RowScale r{};
 
     if (warp == kStoreWarps) {  // fetch
         if (lane == 0) {
@@ -388,9 +409,10 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
             if (ok) mma_commit(acc_full);
         }
     } else {
+        r = row_scale(g, tn * kTileM + (warp & 3) * 32, tm * g.bn);
         const bool ok = tc_wait<false>(acc_full, 0, dead, g.err);
         tc_fence_after();
-        if (ok && a.split == 1) store_tile(g, tmem, tn * kTileM + (warp & 3) * 32, tm * g.bn);
+        if (ok && a.split == 1) store_tile(g, r, tmem, tn * kTileM + (warp & 3) * 32, tm * g.bn);
     }
     if (a.split > 1) {
         const unsigned share = g.bn / a.split, mine0 = rank * share;
@@ -414,25 +436,30 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
         cluster_barrier();
         if (warp < kStoreWarps) {
             const unsigned col = tn * kTileM + l;
-            const bool mine = col < g.n;
-            const float sb = mine ? g.sb[col] : 0.0f, bias = mine && g.bias ? g.bias[col] : 0.0f;
             for (unsigned c = mine0 / 16 * 16 + 16 * (warp >> 2); c < mine0 + share; c += stride) {
                 int v[16];
                 tmem_load16(taddr + c, v);
-                tmem_load_wait();
-                for (unsigned r = 0; r < a.split; ++r) {
-                    if (r == rank) continue;
-                    const int* other = sums + static_cast<unsigned long long>(r) * g.bn * kTileM + l;
+                int o[kMostSplit - 1][16];  // the others', in flight together
+#pragma unroll
+                for (unsigned q = 0; q < kMostSplit - 1; ++q) {
+                    const unsigned from = (rank + 1 + q) % a.split;
+                    const int* other = sums + static_cast<unsigned long long>(from) * g.bn * kTileM + l;
 #pragma unroll
                     for (unsigned j = 0; j < 16; ++j)
-                        if (c + j - mine0 < share) v[j] += __ldcg(other + (c + j) * kTileM);
+                        o[q][j] = q + 1 < a.split && c + j - mine0 < share ? __ldcg(other + (c + j) * kTileM) : 0;
                 }
+                __syncwarp();
+                tmem_load_wait();
+#pragma unroll
+                for (unsigned q = 0; q < kMostSplit - 1; ++q)
+#pragma unroll
+                    for (unsigned j = 0; j < 16; ++j) v[j] += o[q][j];
                 const unsigned row0 = tm * g.bn + c;
 #pragma unroll
                 for (unsigned j = 0; j < 16; ++j)
-                    if (c + j - mine0 < share && mine && row0 + j < g.m) {
-                        const float p = static_cast<float>(v[j]) * (__ldg(g.sa + row0 + j) * sb);
-                        g.out[static_cast<unsigned long long>(row0 + j) * g.n + col] = g.bias ? p + bias : p;
+                    if (c + j - mine0 < share && r.mine && row0 + j < g.m) {
+                        const float p = static_cast<float>(v[j]) * (__ldg(g.sa + row0 + j) * r.scale);
+                        g.out[static_cast<unsigned long long>(row0 + j) * g.n + col] = g.bias ? p + r.bias : p;
                     }
                 __syncwarp();
             }
@@ -497,6 +524,7 @@ matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__
     const unsigned half_bn = g.bn / 2;
     constexpr unsigned a_at = kPairSlices * kTileM * kSliceK;
     const unsigned stage_bytes = a_at + kPairSlices * half_bn * kSliceK;
+    const unsigned copied = kPairSlices * (g.rows + half_bn) * kSliceK;  // of a stage
     const unsigned ntiles = g.tiles_m * g.tiles_n;
     if (threadIdx.x == 0) {
         dead_flag = 0;
@@ -529,12 +557,12 @@ matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__
             for (unsigned i = first; ok && i < ntiles; i += pairs) {
                 unsigned tn, tm;
                 tile_at(i, g, tn, tm);
-                const int row_b = static_cast<int>((2 * tn + rank) * kTileM), row_a = static_cast<int>(tm * g.bn + rank * half_bn);
+                const int row_b = static_cast<int>((2 * tn + rank) * g.rows), row_a = static_cast<int>(tm * g.bn + rank * half_bn);
                 for (unsigned s = 0; s < g.steps; ++s, ++issued, at.next(g.stages)) {
                     if (issued >= g.stages && !(ok = tc_wait<false>(empty + at.slot, at.parity ^ 1, dead, g.err))) break;
                     unsigned char* dst = tiles + at.slot * stage_bytes;
                     const unsigned bar = bars + at.slot * 8;
-                    if (rank == 0) mbar_expect_tx(full + at.slot, 2 * stage_bytes);
+                    if (rank == 0) mbar_expect_tx(full + at.slot, 2 * copied);
                     for (unsigned j = 0; j < kPairSlices; ++j) {
                         const int x = static_cast<int>((s * kPairSlices + j) * kSliceK);
                         tma_load_2d_pair(dst + j * kTileM * kSliceK, &bmap, bar, x, row_b);
@@ -575,11 +603,12 @@ matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__
         unsigned turn = 0;
         for (unsigned i = first; i < ntiles; i += pairs, ++turn) {
             const unsigned half = turn & 1;
-            if (!tc_wait(acc_full + half, (turn >> 1) & 1, dead, g.err)) break;
-            tc_fence_after();
             unsigned tn, tm;
             tile_at(i, g, tn, tm);
-            store_tile(g, tmem + half * g.bn, (2 * tn + rank) * kTileM + (warp & 3) * 32, tm * g.bn);
+            const RowScale r = row_scale(g, (2 * tn + rank) * g.rows + (warp & 3) * 32, tm * g.bn);
+            if (!tc_wait(acc_full + half, (turn >> 1) & 1, dead, g.err)) break;
+            tc_fence_after();
+            store_tile(g, r, tmem + half * g.bn, (2 * tn + rank) * g.rows + (warp & 3) * 32, tm * g.bn);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(in_cta(acc_empty + half, 0));
@@ -633,7 +662,16 @@ void launch_pair(const MatmulQ8Args& a) {
     g.bn = std::min(256u, (a.m + 31) / 32 * 32);
     g.steps = (a.k + kPairSlices * kSliceK - 1) / (kPairSlices * kSliceK);
     g.tiles_m = (a.m + g.bn - 1) / g.bn;
-    g.tiles_n = (a.n + 2 * kTileM - 1) / (2 * kTileM);
+    // With one tile of tokens the weights' way from HBM counts: as many tiles as the
+    // turns that full ones take have room for, of fewer rows (100 x 20000 x 4096:
+    // 24.9 us, with full ones in the same two turns 27.9). A single turn has no
+    // more to gain, and products bound by the tensor cores lose (1000 x 14336 x
+    // 4096: 56 against 54).
+    const unsigned pairs = static_cast<unsigned>(sm_count()) / 2, full = (a.n + 2 * kTileM - 1) / (2 * kTileM);
+    const unsigned long long turns = (static_cast<unsigned long long>(full) * g.tiles_m + pairs - 1) / pairs;
+    const unsigned room = static_cast<unsigned>(turns * pairs / g.tiles_m);  // tiles along the weights
+    g.rows = g.tiles_m == 1 && turns > 1 ? (a.n + 16 * room - 1) / (16 * room) * 8 : kTileM;
+    g.tiles_n = (a.n + 2 * g.rows - 1) / (2 * g.rows);
     const unsigned stage = kPairSlices * (kTileM + g.bn / 2) * kSliceK;  // in each CTA
     g.stages = std::min(8u, 220u * 1024 / stage);
     g.tmem_cols = 32;
@@ -642,11 +680,10 @@ void launch_pair(const MatmulQ8Args& a) {
     g.idesc = 2u << 4 | 1u << 7 | 1u << 10 | (g.bn >> 3) << 17 | (2 * kTileM >> 4) << 24;
     if (static_cast<unsigned long long>(g.tiles_m) * g.tiles_n > 0x7fffffffull)
         fail(VC_ERR_OVERFLOW, "matmul_q8: too many tiles");
-    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, kTileM), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn / 2);
+    const CUtensorMap bmap = slice_map(a.b, a.n, a.k, a.bp, g.rows), amap = slice_map(a.a, a.m, a.k, a.ap, g.bn / 2);
     allow_smem<matmul_q8_pair, kTcSmem>();
-    const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(2 * std::min(ntiles, sms / 2));
+    cfg.gridDim = dim3(2 * std::min(g.tiles_m * g.tiles_n, pairs));
     cfg.blockDim = dim3(kTcThreads);
     cfg.dynamicSmemBytes = g.stages * stage + 1024;
     cfg.stream = stream();
@@ -671,6 +708,7 @@ void launch_split(const MatmulQ8Args& a) {
     g.err = device_error_word();
     const unsigned token_tiles = (a.m + 255) / 256;
     g.bn = ((a.m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    g.rows = kTileM;
     g.steps = (a.k + kSliceK - 1) / kSliceK;
     g.tiles_m = (a.m + g.bn - 1) / g.bn;
     g.tiles_n = (a.n + kTileM - 1) / kTileM;
@@ -678,7 +716,7 @@ void launch_split(const MatmulQ8Args& a) {
     const unsigned ntiles = g.tiles_m * g.tiles_n, sms = static_cast<unsigned>(sm_count());
     g.stages = std::min(8u, 220u * 1024 / stage);
     p.split = 1;
-    while (p.split < 4 && 2 * p.split * ntiles <= sms && g.steps >= 2 * p.split * kSplitSteps) p.split *= 2;
+    while (p.split < kMostSplit && 2 * p.split * ntiles <= sms && g.steps >= 2 * p.split * kSplitSteps) p.split *= 2;
     p.part = (g.steps + p.split - 1) / p.split;
     while (p.split > 1 && (p.split - 1) * p.part >= g.steps) p.split /= 2, p.part = (g.steps + p.split - 1) / p.split;
     g.tmem_cols = 32;
@@ -736,15 +774,15 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
         check_launch("matmul_q8_empty");
     } else {
         // Tiles of 128 weight rows and up to 256 tokens, against the SMs (all in
-        // us, k = 4096): below half of them a tile is shared (64 x 4096: 10.9,
-        // in pairs 13.3; 200 x 8192, at half: 18.2 and 17.9), else pairs walk the
-        // tiles (64 x 11008: 15.0, one CTA a tile 15.9; 4096 x 4096: 54 and 79).
+        // us, k = 4096): below half of them a tile is shared (64 x 4096: 9.5, in
+        // pairs 13.3; 200 x 8192, at half: 17.0 and 17.9), else pairs walk the
+        // tiles (64 x 11008: 15.2, one CTA a tile 16.2; 4096 x 4096: 54 and 79).
         // Up to 8 tokens the weights go straight to registers (8 x 32000: 26, in
         // pairs 30), up to 16 while the tiles are few (16 x 4096: 6.8, shared
-        // 8.3; 16 x 32000 the other way, 33 and 30).
+        // 9.1; 16 x 8192 the other way, 13.1 and 12.2).
         const size_t sms = static_cast<size_t>(sm_count());
         const size_t tiles = ((n + kTileM - 1) / kTileM) * ((m + 255) / 256);
-        if (m <= 8 || (m <= 16 && tiles <= sms)) launch_rows(g);
+        if (m <= 8 || (m <= 16 && 4 * tiles <= sms)) launch_rows(g);
         else if (2 * tiles <= sms) launch_split(g);
         else launch_pair(g);
     }
