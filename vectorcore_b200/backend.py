@@ -87,7 +87,7 @@ def _at(x, elements, dtype, what):
     (None stays None)."""
     if x is None:
         return None
-    if x.dtype != dtype:
+    if x.dtype is not dtype and x.dtype != dtype:
         raise ValueError(f"{what} is {x.dtype}, not {dtype}")
     if x.size < elements:
         raise IndexError(f"{what} has {x.size} elements, {elements} are needed")

@@ -106,7 +106,8 @@ __device__ __forceinline__ Group load_group(const float* p, unsigned g, const Sp
 }
 // The norm's weight, which no output overlaps: read-only loads can be issued
 // ahead of the stores (without that the forward ran at 45% of its speed). It
-// starts on the grid, so a skewed group is four loads.
+// starts on the grid, so a skewed group is four loads (the ends of two of the
+// grid's groups, put together by selects, took as long).
 template <bool SKEWED>
 __device__ __forceinline__ Group load_weight(const float* w, unsigned g, const Span& r) {
     if constexpr (!SKEWED) {
@@ -161,8 +162,13 @@ __device__ __forceinline__ unsigned skew_of(const float* p) {
     return static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(p) >> 2) & 3;
 }
 
+// A row of int8 values up to the next 16 bytes.
+__host__ __device__ __forceinline__ unsigned q8_bytes(unsigned cols) { return (cols + 15) & ~15u; }
+
 // One row a CTA (or a row a warp, blockDim.y of them, for short rows): the row
-// is read once and stays in registers, NV groups a thread.
+// is read once and stays in registers, NV groups a thread; HBM bounds it. 8192 x
+// 8192: 162 us for the norm (6.6 TB/s), 133 in 8 bits (6.55), 61 for the 8 bits
+// alone; rows off the 16-byte grid run at 5.2 TB/s (8000 x 5003: 123 us).
 template <int MODE, bool SKEWED, int NV>
 __global__ void __launch_bounds__(1024)
 norm_kernel(const NormArgs a) {
@@ -234,36 +240,40 @@ norm_kernel(const NormArgs a) {
         const Q8Row o = q8_row(st.amax, rstd);
         if (t == 0) a.scale[row] = o.scale;
         signed char* q = a.q + row * a.pitch;
+        if constexpr (!SKEWED) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const unsigned g = t + i * T;
-            int v[4];
+            for (int i = 0; i < NV; ++i) {
+                const unsigned g = t + i * T;
+                int v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = q8_value(h[i].v[e], o.inv);
-            if (!SKEWED) {
+                for (int e = 0; e < 4; ++e) v[e] = q8_value(h[i].v[e], o.inv);
                 if (g < G) reinterpret_cast<char4*>(q)[g] = make_char4(v[0], v[1], v[2], v[3]);
-            } else {
-                // The row of q starts on the grid. Words of four values take
-                // the end of this lane's group and the beginning of the next
-                // lane's; a warp's two ends go out by bytes.
-                const unsigned lane = t & 31;
-                const unsigned mine = (v[0] & 255) | (v[1] & 255) << 8 | (v[2] & 255) << 16 |
-                                      static_cast<unsigned>(v[3]) << 24;
-                const unsigned next = __shfl_down_sync(0xffffffffu, mine, 1);
-                const unsigned at = 4 * g;  // the word's first element
-                if (lane < 31 && g < G && at + 4 <= a.cols)
-                    *reinterpret_cast<unsigned*>(q + at) = __funnelshift_r(mine, next, 8 * span.skew);
-#pragma unroll
-                for (unsigned e = 0; e < 4; ++e) {
-                    // by bytes: what the words above leave out
-                    const unsigned j = at + e - span.skew;
-                    const bool ahead = e < span.skew;  // in the word of the group before
-                    const bool out = ahead ? lane == 0 || (j & ~3u) + 4 > a.cols : lane == 31 || at + 4 > a.cols;
-                    if (g < G && span.has(g, e) && out) q[j] = static_cast<signed char>(v[e]);
-                }
             }
+            for (unsigned long long j = a.cols + t; j < a.pitch; j += T) q[j] = 0;
+        } else {
+            // The row of q starts on the grid, the groups do not: their bytes meet in
+            // shared memory, those ahead of the row in 16 of its own. (Joined by
+            // shuffles, the ends of warps by bytes, 30000 x 2047 took 127 us without
+            // the norm, now 78.)
+            extern __shared__ __align__(16) signed char rows[];
+            const unsigned bytes = q8_bytes(a.cols);
+            signed char* out = rows + threadIdx.y * (16 + bytes) + 16;
+            if (t < bytes - a.cols) out[a.cols + t] = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const unsigned g = t + i * T;
+                if (g >= G) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    out[static_cast<int>(4 * g + e) - static_cast<int>(span.skew)] =
+                        static_cast<signed char>(q8_value(h[i].v[e], o.inv));
+            }
+            if (T > 32) __syncthreads();
+            else __syncwarp();
+            for (unsigned c = t; c < bytes / 16; c += T)
+                reinterpret_cast<int4*>(q)[c] = reinterpret_cast<const int4*>(out)[c];
+            for (unsigned long long j = bytes + t; j < a.pitch; j += T) q[j] = 0;
         }
-        for (unsigned long long j = a.cols + t; j < a.pitch; j += T) q[j] = 0;
     }
 }
 
@@ -340,7 +350,9 @@ template <int MODE, bool SKEWED, int NV>
 void launch_norm_nv(const NormArgs& a, const RowShape& s) {
     const unsigned long long ctas = (a.rows + s.rows - 1) / s.rows;
     if (ctas > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "rms_norm: too many rows");
-    norm_kernel<MODE, SKEWED, NV><<<static_cast<unsigned>(ctas), dim3(s.threads, s.rows), 0, stream()>>>(a);
+    // trailing zeros of the last group may reach past the row's 16-byte pieces
+    const unsigned smem = MODE != NORM_F32 && SKEWED ? s.rows * (16 + q8_bytes(a.cols)) + 16 : 0;
+    norm_kernel<MODE, SKEWED, NV><<<static_cast<unsigned>(ctas), dim3(s.threads, s.rows), smem, stream()>>>(a);
     check_launch("norm_kernel");
 }
 template <int MODE, bool SKEWED>
