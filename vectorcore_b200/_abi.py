@@ -170,7 +170,9 @@ def check(status: int, what: str = "") -> None:
 
 
 def call(name: str, *args) -> None:
-    check(getattr(lib, name)(*args), name)
+    status = getattr(lib, name)(*args)
+    if status != VC_OK:
+        check(status, name)
 
 
 def shape_arg(shape):

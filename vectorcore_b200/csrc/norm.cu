@@ -51,9 +51,8 @@ __device__ __forceinline__ float warp_amax(float v) {
     return v;
 }
 
-// The row's sum of squares and largest |u|, in every thread of its T threads.
-// fmaxf drops NaN; a NaN (or infinity) shows in the sum, or in `bad` for
-// QUANT_Q8, and poisons the row's scale.
+// The row's sum of squares and largest |u| (no NaN: the callers make it infinity),
+// in every thread of its T threads.
 template <int MODE>
 __device__ __forceinline__ RowStats reduce_row(double sq, float amax, double* ssq, float* smax) {
     const unsigned nw = blockDim.x >> 5;
