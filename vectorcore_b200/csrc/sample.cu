@@ -235,10 +235,12 @@ __device__ __forceinline__ void tell_all(const cg::cluster_group& cluster, Share
 
 // Classes are passed on by fours: v holds those at i .. i + 3, the ones outside
 // the range as masked (-inf), 16 bytes a load where the row allows it. A batch
-// is DEPTH quads, THREADS of them apart, loaded together:
-// f(quads, index of the first quad, loose). Whole warps come along, in the order
-// of the classes, but for the ends that are off the 16-byte grid: these come
-// last, one in the first place of a quad and `loose` true.
+// is DEPTH quads, THREADS of them apart, loaded together, the last one's missing
+// quads masked: f(quads, index of the first quad, loose). Whole warps come along,
+// in the order of the classes, but for the ends that are off the 16-byte grid:
+// these come last, one in the first place of a batch's first quad and `loose`
+// true. One place calls f, which is long: with copies of it for whole batches,
+// single quads and ends 16 x 50000 with top-p took 21.7 us, so 20.1.
 template <unsigned THREADS, int DEPTH, typename F>
 __device__ __forceinline__ void each_batch(const float* __restrict__ x, unsigned begin, unsigned end, F&& f) {
     const unsigned t = threadIdx.x;
@@ -246,28 +248,30 @@ __device__ __forceinline__ void each_batch(const float* __restrict__ x, unsigned
     const unsigned head = min(end, begin + ((4 - skew) & 3));
     const unsigned groups = (end - head) >> 2;
     const float4* body = reinterpret_cast<const float4*>(x + head);
-    const float4 masked = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    unsigned g = t;
-    if constexpr (DEPTH > 1)
-        for (; (g | 31u) + (DEPTH - 1) * THREADS < groups; g += DEPTH * THREADS) {
-            float4 v[DEPTH];
+    // the ends that are off the 16-byte grid, one class a thread of the first warp
+    const unsigned tail = head + 4 * groups, ends = t < 32 ? (head - begin) + (end - tail) : 0;
+    bool loose = false;
+    for (unsigned g = t; !loose; g += DEPTH * THREADS) {
+        float4 v[DEPTH];
+        unsigned i = head + 4 * g;
+        if ((g | 31u) + (DEPTH - 1) * THREADS < groups) {
 #pragma unroll
             for (int j = 0; j < DEPTH; ++j) v[j] = body[g + j * THREADS];
-            f(v, head + 4 * g, std::false_type{});
+        } else {
+#pragma unroll
+            for (int j = 0; j < DEPTH; ++j) v[j] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if ((g & ~31u) < groups) {
+#pragma unroll
+                for (int j = 0; j < DEPTH; ++j)
+                    if (g + j * THREADS < groups) v[j] = body[g + j * THREADS];
+            } else {
+                if (!ends) break;
+                loose = true;
+                i = t < head - begin ? begin + t : tail + t - (head - begin);
+                if (t < ends) v[0].x = x[i];
+            }
         }
-    for (; (g & ~31u) < groups; g += THREADS) {
-        float4 v[1];
-        v[0] = g < groups ? body[g] : masked;
-        f(v, head + 4 * g, std::false_type{});
-    }
-    // the ends that are off the 16-byte grid, one class a thread
-    const unsigned tail = head + 4 * groups, loose = (head - begin) + (end - tail);
-    if (t < 32 && loose) {
-        const unsigned i = t < head - begin ? begin + t : tail + t - (head - begin);
-        float4 v[1];
-        v[0] = masked;
-        if (t < loose) v[0].x = x[i];
-        f(v, i, std::true_type{});
+        f(v, i, loose);
     }
 }
 
@@ -290,10 +294,10 @@ __device__ __forceinline__ First first_quad(const float* __restrict__ x, unsigne
 
 template <unsigned THREADS, int DEPTH, typename F>
 __device__ __forceinline__ void each_quad(const float* x, unsigned begin, unsigned end, F&& f) {
-    each_batch<THREADS, DEPTH>(x, begin, end, [&](const auto& v, unsigned i, auto loose) {
+    each_batch<THREADS, DEPTH>(x, begin, end, [&](const auto& v, unsigned i, bool) {
         constexpr int quads = sizeof(v) / sizeof(float4);
 #pragma unroll
-        for (int j = 0; j < quads; ++j) f(v[j], i + j * 4 * THREADS, loose);
+        for (int j = 0; j < quads; ++j) f(v[j], i + j * 4 * THREADS);
     });
 }
 
@@ -320,9 +324,9 @@ struct Peak {
     float high{-INFINITY};
     unsigned at{0xffffffffu};
     // a batch from i on, all lanes of a warp together
-    template <unsigned THREADS, int N, typename L>
-    __device__ __forceinline__ void see(const float4 (&v)[N], unsigned i, L) {
-        if constexpr (L::value) {
+    template <unsigned THREADS, int N>
+    __device__ __forceinline__ void see(const float4 (&v)[N], unsigned i, bool loose) {
+        if (loose) {
             take_loose(v[0], i);
         } else if (grows(largest(v))) {
 #pragma unroll
@@ -560,7 +564,7 @@ __device__ __noinline__ u64 kth_key(Shared& s, const float* x, unsigned begin, u
     for (unsigned shift = kKeyBits; shift > 0;) {
         shift -= kLevelBits;
         clear_bins(s);
-        each_quad<THREADS, 1>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 1>(x, begin, end, [&](const float4& v, unsigned i) {
             const auto tally = [&](float u, unsigned j) {
                 if (!in_play(u)) return;
                 const u64 key = key_of(u, j);
@@ -634,11 +638,11 @@ sample_kernel(const SampleArgs a) {
             joins(f.v, f.i, w);
             race.start_from(fmaxf(block_max_f(largest(race.scores(w, e)), s), 0.0f));
         }
-        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
+        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, bool loose) {
             constexpr int quads = sizeof(v) / sizeof(float4);
             float4 w[quads], e[quads];
 #pragma unroll
-            for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, decltype(loose)::value);
+            for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, loose);
 #pragma unroll
             for (int j = 0; j < quads; ++j) {
                 w[j] = wt.quick(v[j]);
@@ -656,12 +660,12 @@ sample_kernel(const SampleArgs a) {
         wt.m = fmaxf(capped(block_max_f(largest(f.v), s)), -kLargest);  // no class in play is below that
         if (!first_only) race.start_from(fmaxf(block_max_f(largest(race.scores(wt.quick(f.v), e)), s), 0.0f));
         peak.high = wt.m == 0.0f ? -0x1p-149f : from_ordered(ordered(wt.m) - 1);  // what reaches that maximum is of interest
-        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, auto loose) {
+        each_batch<THREADS, 2>(x, begin, end, [&](const auto& v, unsigned first, bool loose) {
             constexpr int quads = sizeof(v) / sizeof(float4);
             float4 w[quads], e[quads];
             if (!first_only)
 #pragma unroll
-                for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, decltype(loose)::value);
+                for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, loose);
             peak.template see<THREADS>(v, first, loose);
             if (peak.high > wt.m) {  // the whole warp
                 const float less = exp2_quick((wt.m - peak.high) * wt.to_log2);
@@ -676,7 +680,7 @@ sample_kernel(const SampleArgs a) {
         });
     } else {
         each_batch<THREADS, 4>(x, begin, end,
-                               [&](const auto& v, unsigned, auto) { own_peak = fmaxf(own_peak, largest(v)); });
+                               [&](const auto& v, unsigned, bool) { own_peak = fmaxf(own_peak, largest(v)); });
     }
     u64 top = 0;  // (whose index the next pass finds where there is one)
     if (!at_once && in_play(own_peak)) top = key_of(own_peak, 0);
@@ -722,7 +726,7 @@ sample_kernel(const SampleArgs a) {
     if (listing) {
         bool full = false;
         const float least = min_p * (1.0f - kNear);  // the rest of the decision is the race's
-        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i) {
             const float4 w = wt.quick(v);
             total += sum4(w);
             if (!(largest(w) >= least)) return;
@@ -740,7 +744,7 @@ sample_kernel(const SampleArgs a) {
     } else if (!at_once) {
         Shared* one = cluster.map_shared_rank(&s, 0);
         const float from = picking ? cut : most;
-        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i) {
             total += sum4(wt.quick(v));
             if (!(largest(v) >= from)) return;
             find_first(v, i);
@@ -841,7 +845,7 @@ sample_kernel(const SampleArgs a) {
     if (k) {
         const u64 least = kth_key<THREADS>(s, x, begin, end, k);
         double mass = 0.0;
-        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i, auto) {
+        each_quad<THREADS, 2>(x, begin, end, [&](const float4& v, unsigned i) {
             if (!(largest(v) >= key_logit(least))) return;
             const auto keep = [&](float u, unsigned j) {
                 if (!in_play(u) || key_of(u, j) < least) return 0.0f;
@@ -895,7 +899,7 @@ sample_kernel(const SampleArgs a) {
                 if (ahead.of(u, list[c].y)) mass += static_cast<double>(__float2ull_rn(wt.quick(u) * 0x1p40f)) * 0x1p-40;
             }
         } else {
-            each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j, auto) {
+            each_quad<THREADS, 4>(x, begin, end, [&](const float4& v, unsigned j) {
                 if (__any_sync(0xffffffffu, largest(v) >= ahead.x)) mass += sum4(ahead.only(v, j, wt.quick(v)));
             });
         }
