@@ -169,7 +169,8 @@ def test_long_sums_over_rows(backend, rows, cols):
 
 
 @pytest.mark.parametrize("rows,cols", [(7105, 1), (7107, 131), (7111, 33), (3600, 1000), (1801, 1030), (900, 2051),
-                                       (893, 4093), (449, 4099), (450, 8189), (450, 8191), (1000, 8192)])
+                                       (893, 4093), (449, 4099), (450, 8189), (450, 8191), (1000, 8192), (225, 8196),
+                                       (300, 12000), (230, 16380), (4800, 8200), (250, 16384), (250, 16388)])
 @pytest.mark.parametrize("shifted,over", [((), None), ((), "h"), (("dh",), None), (("gh", "w"), "gy"), ((), "gh")])
 def test_gradient_of_many_odd_rows(backend, rows, cols, shifted, over):
     """Rows, or tensors beside h and gy, that start off the 16-byte grid."""

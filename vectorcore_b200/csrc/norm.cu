@@ -536,7 +536,8 @@ void launch_dw_finish(const float* partial, unsigned long long count, unsigned c
     check_launch("norm_dw_finish");
 }
 
-// dh and dw from one pass over h, gy and gh, for rows of up to kRingCols floats:
+// dh and dw from one pass over h, gy and gh, for rows of up to kRingCols floats, or
+// twice as many by pairs of CTAs (below):
 // 16 B an element is all that moves. One CTA an SM walks blocks of R rows (R
 // groups of T threads). A producer warp bulk-copies the blocks of h and gy into a
 // ring of shared-memory stages; gh is loaded a block ahead into registers. A group
@@ -581,22 +582,67 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned b
                  : "memory");
 }
 
-template <bool SKEWED, int NV>
+// Rows of up to twice kRingCols floats: a pair of CTAs has a row, each one half of
+// its columns, and every warp tells both CTAs its part of the dot product. Four
+// places for them go round: before a warp writes to one again, both CTAs have
+// used it. 4000 x 16384 takes 202 us, 5.2 TB/s (dh and dw by themselves 286); 11008
+// columns, 2.7 groups a thread, 4.2 TB/s.
+struct PairSlots {
+    double dot[4][2 * kRingWarps];
+    unsigned long long told[4];
+};
+__device__ __forceinline__ unsigned in_pair(const void* p, unsigned rank) {
+    unsigned a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void pair_tell(PairSlots& s, unsigned place, unsigned warp, double v) {
+    for (unsigned r = 0; r < 2; ++r) {
+        asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_pair(&s.dot[place][warp], r)), "d"(v) : "memory");
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_pair(&s.told[place], r))
+                     : "memory");
+    }
+}
+__device__ __forceinline__ bool pair_wait(unsigned long long* bar, unsigned parity, unsigned* err) {
+    for (long long i = 0; i < kWaitPolls / 8; ++i) {
+        unsigned ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, "
+            "1, 0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_addr(bar)), "r"(parity), "r"(kWaitHintNs)
+            : "memory");
+        if (ok) return true;
+    }
+    atomicOr(err, kErrWaitTimeout);
+    return false;
+}
+__device__ __forceinline__ void pair_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <bool SKEWED, bool PAIRED, int NV>
 __global__ void __launch_bounds__(kRingThreads + (SKEWED ? 64 : 32), 1)
 norm_bwd_ring(const RingArgs a) {
+    static_assert(!(SKEWED && PAIRED), "pairs have whole groups");
     extern __shared__ __align__(128) float ring[];
     __shared__ unsigned long long full[kRingMaxStages], empty[kRingMaxStages], clean[SKEWED ? kRingMaxStages : 1];
     __shared__ double slots[3][kRingWarps];
     __shared__ unsigned dead_flag;
     volatile unsigned* dead = &dead_flag;
     const unsigned warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const unsigned cols = a.n.cols, block_floats = a.R * a.pitch;
+    __shared__ PairSlots pair;  // not in the kernels of single CTAs
+    // this CTA's columns of a row, c0 on, and its place among the CTAs or pairs
+    const unsigned length = a.n.cols, half = PAIRED ? blockIdx.x & 1 : 0, c0 = half * a.pitch;
+    const unsigned cols = PAIRED ? (half ? length - a.pitch : a.pitch) : length;
+    const unsigned place = PAIRED ? blockIdx.x >> 1 : blockIdx.x, places = PAIRED ? gridDim.x >> 1 : gridDim.x;
+    const unsigned block_floats = a.R * a.pitch;
     const unsigned stage_floats = 2 * block_floats;
     // this CTA's class and its rows' skew, its first block and the step to the next
-    const unsigned classes = SKEWED ? a.classes : 1, kind = SKEWED ? blockIdx.x % classes : 0;
+    const unsigned classes = SKEWED ? a.classes : 1, kind = SKEWED ? place % classes : 0;
     const Span span{SKEWED ? (kind * cols) & 3 : 0, cols};
-    const unsigned long long begin = blockIdx.x / classes;
-    const unsigned step = gridDim.x / classes;
+    const unsigned long long begin = place / classes;
+    const unsigned step = places / classes;
     const auto row_at = [&](unsigned long long b, unsigned r) { return (b * a.R + r) * classes + kind; };
     if (threadIdx.x == 0) {
         dead_flag = 0;
@@ -605,9 +651,12 @@ norm_bwd_ring(const RingArgs a) {
             if (SKEWED) mbar_init(clean + s, 1);
             mbar_init(empty + s, a.R * a.T / 32);
         }
+        if (PAIRED)
+            for (unsigned s = 0; s < 4; ++s) mbar_init(pair.told + s, 2 * kRingWarps);
         mbar_fence_init();
     }
     __syncthreads();
+    if (PAIRED) pair_barrier();
 
     if (warp == kRingWarps) {  // producer
         unsigned issued = 0;
@@ -627,8 +676,8 @@ norm_bwd_ring(const RingArgs a) {
                 const unsigned bytes = rows * cols * sizeof(float);
                 if (lane == 0) {
                     mbar_expect_tx(full + slot, 2 * bytes);
-                    bulk_copy(at, a.n.h + row * cols, bytes, full + slot);
-                    bulk_copy(at + block_floats, a.n.gy + row * cols, bytes, full + slot);
+                    bulk_copy(at, a.n.h + row * length + c0, bytes, full + slot);
+                    bulk_copy(at + block_floats, a.n.gy + row * length + c0, bytes, full + slot);
                 }
             } else {  // a row a lane
                 const unsigned long long row = row_at(b, lane), first = row * cols;
@@ -684,7 +733,7 @@ norm_bwd_ring(const RingArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             dw[i] = Group{};
-            w[i] = t + i * a.T < G ? load_weight<SKEWED>(a.n.w, t + i * a.T, span) : Group{};
+            w[i] = t + i * a.T < G ? load_weight<SKEWED>(a.n.w + c0, t + i * a.T, span) : Group{};
         }
         // A thread's columns of a partial row, whose own rows are off the grid too.
         const auto put = [&](float* out, unsigned at_c, const Group& v) {
@@ -698,7 +747,7 @@ norm_bwd_ring(const RingArgs a) {
             }
         };
         unsigned segment = 0;
-        const double by_cols = 1.0 / cols;
+        const double by_cols = 1.0 / length;
         const auto row_of = [&](unsigned long long b) { return row_at(b, group); };
         Group up[NV];  // gh of the row whose dot product was added up last
         float s_of = 0.0f;  // and its rstd
@@ -713,7 +762,7 @@ norm_bwd_ring(const RingArgs a) {
                 const unsigned c = t + i * a.T;
                 up[i] = Group{};
                 if (mine && a.n.gh && c < G) {
-                    const float* gh = a.n.gh + row * cols;
+                    const float* gh = a.n.gh + row * length + c0;
                     if (SKEWED && row + 1 == a.n.rows) up[i] = load_group<SKEWED>(gh, c, span);
                     else up[i] = group_of(reinterpret_cast<const float4*>(gh - span.skew)[c]);
                 }
@@ -736,13 +785,22 @@ norm_bwd_ring(const RingArgs a) {
                 }
             }
             dot = warp_sum(dot);
-            if (lane == 0) slots[i_th % 3][warp] = dot;
+            if (lane == 0) {
+                if constexpr (PAIRED) pair_tell(pair, i_th & 3, half * kRingWarps + warp, dot);
+                else slots[i_th % 3][warp] = dot;
+            }
         };
         // dh of block b's row, whose gh and rstd are given.
         const auto give = [&](unsigned long long b, unsigned i_th, const Group (&gh)[NV], float s) {
             const unsigned slot = i_th % a.stages;
             const unsigned long long row = row_of(b);
-            const double dot = warp_sum(lane < a.T >> 5 ? slots[i_th % 3][group * (a.T >> 5) + lane] : 0.0);
+            double dot;
+            if constexpr (PAIRED) {
+                if (!*dead && !pair_wait(pair.told + (i_th & 3), (i_th >> 2) & 1, a.err)) *dead = 1;
+                dot = warp_sum(pair.dot[i_th & 3][lane]);
+            } else {
+                dot = warp_sum(lane < a.T >> 5 ? slots[i_th % 3][group * (a.T >> 5) + lane] : 0.0);
+            }
             const float c = static_cast<float>(dot * by_cols) * (s * s);
             if (row < a.n.rows) {
                 const float* at = ring + slot * stage_floats + group * a.pitch;
@@ -754,7 +812,7 @@ norm_bwd_ring(const RingArgs a) {
                     Group o;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o.v[e] = fmaf(s, fmaf(-h.v[e], c, g.v[e] * w[i].v[e]), gh[i].v[e]);
-                    float* dh = a.n.dh + row * cols;
+                    float* dh = a.n.dh + row * length + c0;
                     if (!SKEWED || (at_c > 0 && at_c < G - 1))
                         __stcs(reinterpret_cast<float4*>(dh - span.skew) + at_c, make_float4(o.v[0], o.v[1], o.v[2], o.v[3]));
                     else
@@ -773,7 +831,7 @@ norm_bwd_ring(const RingArgs a) {
             for (int i = 0; i < NV; ++i) gh[i] = up[i];
             const float s = s_of;
             if ((used + 1) % kDwRows == 0 && segment + 1 < a.segments) {  // enough float additions
-                float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
+                float* out = a.partial + ((static_cast<unsigned long long>(place) * (a.segments - 1) + segment) * a.R + group) * length + c0;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
                     put(out, t + i * a.T, dw[i]);
@@ -782,12 +840,12 @@ norm_bwd_ring(const RingArgs a) {
                 ++segment;
             }
             if (b + step < a.blocks) take(b + step, used + 1);
-            if (a.T > 32) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(a.T) : "memory");
-            else __syncwarp();
+            if (PAIRED || a.T == 32) __syncwarp();
+            else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(a.T) : "memory");
             give(b, used, gh, s);
         }
         for (; works && segment + 1 < a.segments; ++segment) {  // CTAs with fewer blocks
-            float* out = a.partial + ((static_cast<unsigned long long>(blockIdx.x) * (a.segments - 1) + segment) * a.R + group) * cols;
+            float* out = a.partial + ((static_cast<unsigned long long>(place) * (a.segments - 1) + segment) * a.R + group) * length + c0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) put(out, t + i * a.T, Group{});
         }
@@ -797,55 +855,73 @@ norm_bwd_ring(const RingArgs a) {
         for (int i = 0; i < NV; ++i)
             if (works) put(ring + group * cols, t + i * a.T, dw[i]);
         asm volatile("bar.sync 15, %0;" ::"n"(kRingThreads) : "memory");
-        float* out = a.partial + (static_cast<unsigned long long>(gridDim.x) * (a.segments - 1) * a.R + blockIdx.x) * cols;
+        float* out = a.partial + (static_cast<unsigned long long>(places) * (a.segments - 1) * a.R + place) * length + c0;
         for (unsigned c = threadIdx.x; c < cols; c += kRingThreads) {
             float sum = ring[c];
             for (unsigned r = 1; r < a.R; ++r) sum += ring[r * cols + c];
             out[c] = sum;
         }
     }
+    if (PAIRED) {
+        __syncwarp();
+        pair_barrier();  // nobody leaves while its shared memory may be written
+    }
 }
 
-template <bool SKEWED, int NV>
+template <bool SKEWED, bool PAIRED, int NV>
 void launch_ring_nv(const RingArgs& a, unsigned ctas, unsigned smem) {
-    allow_smem<norm_bwd_ring<SKEWED, NV>, kRingSmem>();
-    norm_bwd_ring<SKEWED, NV><<<ctas, kRingThreads + (SKEWED ? 64 : 32), smem, stream()>>>(a);
+    allow_smem<norm_bwd_ring<SKEWED, PAIRED, NV>, kRingSmem>();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kRingThreads + (SKEWED ? 64 : 32));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIRED ? 2 : 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    VC_CUDA(cudaLaunchKernelEx(&cfg, norm_bwd_ring<SKEWED, PAIRED, NV>, a));
 }
 template <bool SKEWED>
 void launch_ring(const RingArgs& a, unsigned groups, unsigned ctas, unsigned smem) {
     const unsigned per = (groups + a.T - 1) / a.T;
-    if (per <= 1) launch_ring_nv<SKEWED, 1>(a, ctas, smem);
-    else if (per <= 2) launch_ring_nv<SKEWED, 2>(a, ctas, smem);
-    else launch_ring_nv<SKEWED, 4>(a, ctas, smem);
+    if (per <= 1) launch_ring_nv<SKEWED, false, 1>(a, ctas, smem);
+    else if (per <= 2) launch_ring_nv<SKEWED, false, 2>(a, ctas, smem);
+    else launch_ring_nv<SKEWED, false, 4>(a, ctas, smem);
 }
 
 // The fused pass, where it applies; false, having launched nothing, otherwise.
 bool try_bwd_ring(const NormBwdArgs& n, float* dw) {
     if (!aligned16(n.h) || !aligned16(n.gy) || !aligned16(n.dh) || (n.gh && !aligned16(n.gh))) return false;
-    const bool skewed = n.cols % 4 != 0 || !aligned16(n.w);
-    const unsigned groups = skewed ? (n.cols + 3 + 3) / 4 : n.cols / 4;  // at most
+    const bool skewed = n.cols % 4 != 0 || !aligned16(n.w), paired = !skewed && n.cols > kRingCols;
+    // groups of a row, or of a CTA's half of it, at most
+    const unsigned groups = skewed ? (n.cols + 3 + 3) / 4 : paired ? (n.cols / 4 + 1) / 2 : n.cols / 4;
     // (a row's copy may reach three floats into the next row)
     if (groups > kRingCols / 4 || n.cols < 4) return false;
     RingArgs a{};
     a.n = n;
     // up to four groups a thread; rows of 2^n floats and their neighbours off the
     // grid need one group more, and 3 or 5 rows a block instead of half of 4 or 8
-    for (a.R = 16; a.R > 1 && 4 * (kRingThreads / a.R / 32 * 32) < groups;) a.R = skewed ? a.R - 1 : a.R / 2;
+    for (a.R = paired ? 1 : 16; a.R > 1 && 4 * (kRingThreads / a.R / 32 * 32) < groups;) a.R = skewed ? a.R - 1 : a.R / 2;
     a.T = kRingThreads / a.R / 32 * 32;
     a.classes = n.cols % 4 == 0 ? 1 : n.cols % 2 == 0 ? 2 : 4;
-    a.pitch = skewed ? 4 * groups : n.cols;
-    const unsigned ctas = static_cast<unsigned>(sm_count()) / a.classes * a.classes, step = ctas / a.classes;
+    a.pitch = skewed || paired ? 4 * groups : n.cols;
+    const unsigned share = a.classes * (paired ? 2 : 1);
+    const unsigned step = static_cast<unsigned>(sm_count()) / share, ctas = step * share, places = step * a.classes;
     a.blocks = ((n.rows + a.classes - 1) / a.classes + a.R - 1) / a.R;
     if (a.blocks < 3ull * step) return false;
     const unsigned stage = 2 * a.R * a.pitch * sizeof(float);
     a.stages = std::min(kRingMaxStages, kRingSmem / stage);
     const unsigned long long most = (a.blocks + step - 1) / step;
     a.segments = static_cast<unsigned>((most + kDwRows - 1) / kDwRows);
-    const unsigned long long partial_rows = static_cast<unsigned long long>(ctas) * ((a.segments - 1) * a.R + 1);
+    const unsigned long long partial_rows = static_cast<unsigned long long>(places) * ((a.segments - 1) * a.R + 1);
     Scratch partial(partial_rows * n.cols * sizeof(float));
     a.partial = partial.as<float>();
     a.err = device_error_word();
-    if (skewed) launch_ring<true>(a, groups, ctas, a.stages * stage);
+    if (paired) launch_ring_nv<false, true, 4>(a, ctas, a.stages * stage);
+    else if (skewed) launch_ring<true>(a, groups, ctas, a.stages * stage);
     else launch_ring<false>(a, groups, ctas, a.stages * stage);
     check_launch("norm_bwd_ring");
     launch_dw_finish(a.partial, partial_rows, n.cols, dw);
