@@ -931,18 +931,18 @@ void launch_rows(const SampleArgs& a, unsigned rows, unsigned C) {
 }
 
 // Up to here four CTAs of 256 threads an SM are faster than two of 512: a row is
-// mostly barriers (512 rows of 4000 classes: 22 us against 28; 256 of 128000,
-// the other way, 98 against 105).
+// mostly barriers (512 rows of 4000 classes: 21 us against 26; 256 of 128000,
+// the other way, 96 against 88).
 constexpr bool vocab_fits_four(unsigned vocab) { return vocab <= 16384; }
 
 // Few rows are bound by the latency of their passes and barriers: as many CTAs a
 // row, of 512 threads, as leave each an SM of its own and 1600 classes (16 x 8000:
-// 11.6 us, with 3200 classes 12.8), or half an SM and 4800 (64 x 128000: 45 us
-// against 50 alone on an SM; 140 x 8000 the other way, 21 against 18). With more
+// 11.9 us, with 3200 classes 12.4), or half an SM and 4800 (64 x 128000: 45 us
+// against 67 alone on an SM; 140 x 8000 the other way, 19.5 against 16.9). With more
 // rows, two CTAs an SM, so that one's passes run through the other's barriers, and
 // as many of them a row (which is read more than once where there are filters) as
 // keep the rows that run together within 48 MB: beyond that L2 loses a row between
-// its passes (256 x 128000: 98 us, with half as many CTAs a row 106).
+// its passes (256 x 128000: 88 us, with half as many CTAs a row 99).
 void launch_sample(SampleArgs& a, std::size_t rows) {
     const u64 sms = static_cast<unsigned>(sm_count());
     const bool filtered = a.top_k || a.top_p || a.min_p;
