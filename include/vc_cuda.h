@@ -504,13 +504,13 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
  * is the class with the largest w / noise, the lowest index of equal ones:
  * class i with probability w_i / (sum of w in the race). A temperature that is
  * not above 0 takes the first class in order (greedy; logprob at temperature
- * 1). NaN and -inf logits are masked: never drawn; +inf counts as the largest
- * float; classes whose w is below 2^-126 are not drawn. Masses are within 2^-14
- * relative, so a class that near the edge of top_p may fall on either side.
- * logprob is the token's under softmax(logits / temperature) before the filters.
- * A row with every class masked gives token -1 and logprob NaN. The same inputs
- * give the same tokens, whatever else runs. vocab <= 2^23, larger fails with
- * VC_ERR_OVERFLOW. */
+ * 1); one below 2^-126 counts as 2^-126. NaN and -inf logits are masked: never
+ * drawn; +inf counts as the largest float; classes whose w is below 2^-126 are
+ * not drawn. Masses are within 2^-14 relative, so a class that near the edge of
+ * top_p may fall on either side. logprob is the token's under
+ * softmax(logits / temperature) before the filters. A row with every class
+ * masked gives token -1 and logprob NaN. The same inputs give the same tokens,
+ * whatever else runs. vocab <= 2^23, larger fails with VC_ERR_OVERFLOW. */
 vc_status vc_cuda_sample(const float* logits, size_t logits_stride, const float* noise, size_t noise_stride,
                          const float* temperature, const int64_t* top_k, const float* top_p, const float* min_p,
                          size_t rows, size_t vocab, int64_t* token, float* logprob);

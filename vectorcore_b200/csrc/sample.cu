@@ -111,8 +111,10 @@ __device__ __forceinline__ float quotient_quick(float a, float b) {
 }
 
 // How a row weighs its classes. +inf counts as the largest float, so that no
-// difference of two logits in play is NaN.
-constexpr float kLargest = 3.402823466e38f;
+// difference of two logits in play is NaN. A temperature below the smallest
+// normal float counts as that one: log2(e) / T would be infinite, and 0 (the
+// maximum's distance) times it NaN.
+constexpr float kLargest = 3.402823466e38f, kColdest = 0x1p-126f;
 __device__ __forceinline__ float capped(float x) {  // NaN stays
     float y;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(kLargest));
@@ -123,7 +125,7 @@ struct Weigh {
     float to_log2;  // log2(e) / T
     __device__ __forceinline__ void set(float top, float temperature) {
         m = capped(top);
-        t = fminf(temperature, kLargest);
+        t = fminf(fmaxf(temperature, kColdest), kLargest);
         to_log2 = static_cast<float>(1.4426950408889634 / static_cast<double>(t));
     }
     __device__ __forceinline__ float distance(float x) const {
