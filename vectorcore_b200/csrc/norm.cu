@@ -692,6 +692,7 @@ norm_bwd_ring(const RingArgs a) {
                     }
                 }
                 const unsigned all = __reduce_add_sync(0xffffffffu, floats);
+                __syncwarp();  // lane 0 arrives for the other lanes' stores too
                 if (lane == 0) mbar_expect_tx(full + slot, 2 * all * sizeof(float));
                 __syncwarp();
                 if (have) {
