@@ -38,3 +38,28 @@ def test_temperatures_below_the_normal_floats_count_as_the_smallest(backend):
         token, logprob = run(backend, x, noise, [{"temperature": t, **filters} for t in cold])
         for i, t in enumerate(cold):
             R.Row(x[i], noise[i], max(t, 2.0 ** -126), **filters).check(int(token[i]), float(logprob[i]), f"{t} {filters}")
+
+
+@pytest.mark.parametrize("steps", [1, 5, 7, 11, 13, 17, 23, 29])
+def test_a_maximum_that_grows_all_along_a_long_row(backend, steps):
+    """The longest rows, one CTA a row, every batch of classes above the one
+    before it. An early class and a late one are 3e-6 apart in the race, where
+    the definition's e^d (2^-22), division and the noise's own rounding (2^-24
+    each) leave 4e-7; d is exact."""
+    rows, vocab, batch = 149, 1 << 23, 4096
+    batches = vocab // batch
+    step = steps * 2.0 ** -11  # all distances exact
+    x = (np.arange(vocab) // batch * step).astype(np.float32)
+    up, early, late = backend.upload, 40, vocab - batch + 40
+    dx = up(x)
+    total = batch * np.exp(-step * np.arange(batches)).sum()
+    for winner, factor in ((early, 1 - 3e-6), (late, 1 + 3e-6)):
+        noise = np.full(vocab, 1e9, np.float32)
+        noise[late], noise[early] = 1.0, np.exp(-step * (batches - 1)) * factor
+        token, logprob = backend.sample(dx, up(noise), rows, vocab, row_stride=0, noise_stride=0)
+        assert (backend.download(token) == winner).all()
+        # rounding as in _lm_ref.Row.check, no distance above the longest
+        want = (step * (batches - 1) if winner == early else 0.0) * -1.0 - np.log(total)
+        worst = step * (batches - 1)
+        bound = R.U * (8 * worst + 8 + 4 * np.log(total) + abs(want))
+        assert (np.abs(backend.download(logprob) - want) <= bound).all()

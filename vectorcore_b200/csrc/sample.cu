@@ -31,8 +31,9 @@
 // order's key, (ordered logit bits, ~index), 11 bits each, and then a list too.
 //
 // Without top-k and min-p a row is read once from HBM, the sum and the race
-// running against the maximum so far; with them, once for its maximum and once,
-// from L1 or L2, for the sum and the list.
+// running against the maximum so far, or one at most 2^8 in weight below it;
+// with them, once for its maximum and once, from L1 or L2, for the sum and the
+// list.
 //
 // Weights come in two makes. `weight` is the definition in float: one
 // subtraction, one division, expf. `quick` is one product and ex2.approx,
@@ -65,6 +66,7 @@ constexpr unsigned kKeyBits = 32 + kIndexBits;
 constexpr unsigned kLevelBits = 11;    // of the key a histogram resolves
 constexpr unsigned kMaxCluster = 8;
 constexpr float kNear = 0x1p-14f;      // quick results this near to each other are decided exactly
+constexpr float kGrown = 8.0f;         // log2 by which the maximum of the one pass grows before weights follow it
 
 struct SampleArgs {
     const float* logits;
@@ -669,7 +671,10 @@ sample_kernel(const SampleArgs a) {
 #pragma unroll
                 for (int j = 0; j < quads; ++j) e[j] = race.numbers(first + j * 4 * THREADS, end, loose);
             peak.template see<THREADS>(v, first, loose);
-            if (peak.high > wt.m) {  // the whole warp
+            // The whole warp; not for every new maximum, since each time rounds the
+            // sum and the race once more: what was there at first has left the
+            // floats' range (2^-126) after 16 times.
+            if ((peak.high - wt.m) * wt.to_log2 > kGrown) {
                 const float less = exp2_quick((wt.m - peak.high) * wt.to_log2);
                 total *= less;
                 race.rescale(less);
