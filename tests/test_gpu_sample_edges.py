@@ -63,3 +63,27 @@ def test_a_maximum_that_grows_all_along_a_long_row(backend, steps):
         worst = step * (batches - 1)
         bound = R.U * (8 * worst + 8 + 4 * np.log(total) + abs(want))
         assert (np.abs(backend.download(logprob) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("vocab", [10, 300, 4097, 20000, 50000])
+@pytest.mark.parametrize("setting", [{"temperature": 0.0}, {}, {"top_k": 1}, {"top_k": 2}, {"top_k": 600},
+                                     {"top_k": 600, "top_p": 0.4}, {"top_p": 0.4}, {"min_p": 0.5},
+                                     {"top_p": 0.4, "min_p": 0.5}])
+def test_infinity_counts_as_the_largest_float(backend, vocab, setting):
+    """Equal ones are ordered by index alone, near to each other and far apart."""
+    rng = np.random.default_rng(vocab)
+    big, rows = np.finfo(np.float32).max, 6
+    x = rng.normal(size=(rows, vocab)).astype(np.float32)
+    x[0, 0], x[0, -1] = big, np.inf
+    x[1, 0], x[1, -1] = np.inf, big
+    x[2, 1:3] = np.inf, big
+    x[3, -3:-1] = big, np.inf
+    x[4, ::2], x[4, 1::2] = big, np.inf
+    x[5, ::3] = np.where(rng.random(x[5, ::3].size) < 0.5, big, np.inf)
+    noise = rng.exponential(size=x.shape).astype(np.float32)
+    for rows_again in (1, 30):  # 180 rows take the other launch shapes
+        xs, es = np.tile(x, (rows_again, 1)), np.tile(noise, (rows_again, 1))
+        token, logprob = run(backend, xs, es, [setting] * len(xs))
+        for i in range(rows):
+            R.Row(np.minimum(x[i], big), noise[i], **setting).check(int(token[i]), float(logprob[i]), f"row {i}")
+        assert (token.reshape(-1, rows) == token[:rows]).all()

@@ -83,9 +83,10 @@ struct SampleArgs {
     float* logprob;
 };
 
-// Floats in order as unsigned integers; -0 counts as +0.
+constexpr float kLargest = 3.402823466e38f;
+// Floats in order as unsigned integers; -0 counts as +0, +inf as the largest.
 __device__ __forceinline__ unsigned ordered(float x) {
-    const unsigned u = __float_as_uint(x + 0.0f);
+    const unsigned u = __float_as_uint(fminf(x, kLargest) + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float from_ordered(unsigned u) {
@@ -116,7 +117,7 @@ __device__ __forceinline__ float quotient_quick(float a, float b) {
 // difference of two logits in play is NaN. A temperature below the smallest
 // normal float counts as that one: log2(e) / T would be infinite, and 0 (the
 // maximum's distance) times it NaN.
-constexpr float kLargest = 3.402823466e38f, kColdest = 0x1p-126f;
+constexpr float kColdest = 0x1p-126f;
 __device__ __forceinline__ float capped(float x) {  // NaN stays
     float y;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(kLargest));
@@ -590,8 +591,10 @@ __device__ __noinline__ u64 kth_key(Shared& s, const float* x, unsigned begin, u
 struct Ahead {
     float x;
     unsigned i;
-    __device__ __forceinline__ explicit Ahead(u64 key) : x(key_logit(key)), i(key_index(key)) {}
-    __device__ __forceinline__ bool of(float u, unsigned j) const { return u > x || (u == x && j < i); }
+    float over;  // what is above it is ahead of it: nothing of the largest float, which +inf equals
+    __device__ __forceinline__ explicit Ahead(u64 key)
+        : x(key_logit(key)), i(key_index(key)), over(x < kLargest ? x : INFINITY) {}
+    __device__ __forceinline__ bool of(float u, unsigned j) const { return u > over || (u >= x && j < i); }
     // a quad's weights, 0 for the ones that are not
     __device__ __forceinline__ float4 only(const float4& v, unsigned j, const float4& w) const {
         return make_float4(of(v.x, j) ? w.x : 0.0f, of(v.y, j + 1) ? w.y : 0.0f, of(v.z, j + 2) ? w.z : 0.0f,
@@ -688,10 +691,11 @@ sample_kernel(const SampleArgs a) {
     } else {
         each_batch<THREADS, 4>(x, begin, end,
                                [&](const auto& v, unsigned, bool) { own_peak = fmaxf(own_peak, largest(v)); });
+        own_peak = capped(own_peak);
     }
     u64 top = 0;  // (whose index the next pass finds where there is one)
     if (!at_once && in_play(own_peak)) top = key_of(own_peak, 0);
-    if (peak.at != 0xffffffffu) top = key_of(peak.high < kLargest ? peak.high : x[peak.at], peak.at);
+    if (peak.at != 0xffffffffu) top = key_of(peak.high, peak.at);
     top = block_max64(top, s);
     if (t == 0) s.listed = s.picked = 0, s.first = 0xffffffffu;
     cluster.barrier_wait(std::move(begun));  // every CTA has begun: its shared memory may be written
@@ -716,9 +720,9 @@ sample_kernel(const SampleArgs a) {
         }
         return;
     }
-    const float most = key_logit(top), high = capped(most);
-    if (at_once) total *= exp2_quick((wt.m - high) * wt.to_log2);
-    wt.m = high;
+    const float most = key_logit(top);
+    if (at_once) total *= exp2_quick((wt.m - most) * wt.to_log2);
+    wt.m = most;
 
     // The classes that may be left are listed: of a small k, from the k-th largest
     // of the groups' maxima on, and by the first CTA; of min-p, the ones that reach
@@ -727,7 +731,7 @@ sample_kernel(const SampleArgs a) {
     if (few && k <= groups) cut = kth_of<THREADS>(s, s.group, groups, static_cast<unsigned>(k));
     const bool picking = in_play(cut), listing = min_p > 0.0f && !k;
     const auto find_first = [&](const float4& v, unsigned i) {
-        const unsigned at = v.x == most ? i : v.y == most ? i + 1 : v.z == most ? i + 2 : v.w == most ? i + 3 : 0xffffffffu;
+        const unsigned at = v.x >= most ? i : v.y >= most ? i + 1 : v.z >= most ? i + 2 : v.w >= most ? i + 3 : 0xffffffffu;
         if (at != 0xffffffffu) atomicMin(&s.first, at);
     };
     if (listing) {
