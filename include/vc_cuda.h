@@ -486,9 +486,10 @@ vc_status vc_cuda_quantize_q8(const float* x, size_t x_stride, size_t rows, size
 
 /* out [m, n] = (a b^T) * (a_scale[i] * b_scale[j]) + bias[j] for q8 matrices
  * a [m, k] (activations, a scale for each token) and b [n, k] (weights, a
- * scale for each output channel); bias may be NULL. The sums are exact 32-bit
- * integers: k <= 131071, larger fails with VC_ERR_OVERFLOW. k = 0 gives the
- * bias alone. */
+ * scale for each output channel); bias may be NULL. A product of two scales may
+ * be too small or too large for a float: only the result has to fit one. The
+ * sums are exact 32-bit integers: k <= 131071, larger fails with
+ * VC_ERR_OVERFLOW. k = 0 gives the bias alone. */
 vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scale, const int8_t* b, size_t b_pitch,
                             const float* b_scale, const float* bias, size_t m, size_t n, size_t k, float* out);
 

@@ -5,6 +5,10 @@
 //
 // The sums are 32-bit integers, so they are exact and do not depend on the
 // order of the additions (|a * b| <= 2^14, hence k <= 131071).
+//
+// A sum is scaled by one float, the product of its two scales. Where that leaves
+// the normal floats, though the result need not, the sum and both scales are
+// multiplied in double, which holds all of them.
 #include "vc_internal.cuh"
 
 namespace vc {
@@ -22,6 +26,17 @@ struct MatmulQ8Args {
     float* out;
     unsigned m, n, k;
 };
+
+// sum * (sa * sb). The products of a 0 (a row of zeros) are left as they are, those
+// of an infinity or a NaN come out the same either way.
+__device__ __forceinline__ float scaled(int sum, float sa, float sb) {
+    const float s = sa * sb;
+    if (!(fabsf(s) >= 0x1p-126f && fabsf(s) < INFINITY) && sa != 0.0f && sb != 0.0f)
+        return static_cast<float>(static_cast<double>(sum) * (static_cast<double>(sa) * static_cast<double>(sb)));
+    return static_cast<float>(sum) * s;
+}
+// Any two scales of which this holds have a product that is only rounded.
+__device__ __forceinline__ bool is_plain(float s) { return s == 0.0f || (fabsf(s) >= 0x1p-63f && fabsf(s) <= 0x1p63f); }
 
 // ---- few tokens -------------------------------------------------------------------
 //
@@ -110,16 +125,19 @@ matmul_q8_rows(const MatmulQ8Args g) {
         sums[warp][r + 8][8 * i + 2 * q] = acc[i][2];
         sums[warp][r + 8][8 * i + 2 * q + 1] = acc[i][3];
     }
+    // one output a thread; what scales it is fetched while the sums meet
+    static_assert(16 * 8 * NT <= kRowsWarps * 32);
+    const unsigned token = threadIdx.x >> 4, row = threadIdx.x & 15;
+    const bool mine = token < min(g.m, 8u * NT) && row0 + row < g.n;
+    const float sa = mine ? __ldg(g.sa + token) : 0.0f, sb = mine ? __ldg(g.sb + row0 + row) : 0.0f;
+    const float bias = mine && g.bias ? __ldg(g.bias + row0 + row) : 0.0f;
     __syncthreads();
-    for (unsigned i = threadIdx.x; i < 16 * 8 * NT; i += kRowsWarps * 32) {
-        const unsigned token = i >> 4, row = i & 15;
-        if (token >= g.m || row0 + row >= g.n) continue;
-        int sum = 0;
+    if (!mine) return;
+    int sum = 0;
 #pragma unroll
-        for (unsigned v = 0; v < kRowsWarps; ++v) sum += sums[v][row][token];
-        const float p = static_cast<float>(sum) * (g.sa[token] * g.sb[row0 + row]);
-        g.out[static_cast<unsigned long long>(token) * g.n + row0 + row] = g.bias ? p + g.bias[row0 + row] : p;
-    }
+    for (unsigned v = 0; v < kRowsWarps; ++v) sum += sums[v][row][token];
+    const float p = scaled(sum, sa, sb);
+    g.out[static_cast<unsigned long long>(token) * g.n + row0 + row] = g.bias ? p + bias : p;
 }
 
 void launch_rows(const MatmulQ8Args& g) {
@@ -194,6 +212,14 @@ __device__ __forceinline__ void tmem_load16(unsigned taddr, int (&v)[16]) {
           "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
         : "r"(taddr));
 }
+__device__ __forceinline__ int tmem_load1(unsigned taddr) {
+    int v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(v)
+                 : "r"(taddr)
+                 : "memory");
+    return v;
+}
 __device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -252,27 +278,48 @@ __device__ __forceinline__ void tile_at(unsigned i, const TcArgs& g, unsigned& t
 // What a store thread needs beside the sums of its weight row, loaded while the
 // sums are on their way: they come from HBM, and fetched after them, with the other
 // CTAs' sums one after another, 256 x 4096 x 4096 took 15.8 us, so 13.0. The tokens'
-// scales are read later, from L1.
+// scales are looked at then too, and read later, from L1.
 struct RowScale {
     bool mine;
     float scale, bias;
 };
-__device__ __forceinline__ RowScale row_scale(const TcArgs& g, unsigned first, unsigned row0) {
-    const unsigned lane = threadIdx.x & 31, col = first + lane, token = row0 + 8 * lane;
-    RowScale r{col < g.n && (threadIdx.x >> 5 & 3) * 32 + lane < g.rows, 0.0f, 0.0f};
+__device__ __forceinline__ RowScale row_scale(const TcArgs& g, unsigned first) {
+    const unsigned lane = threadIdx.x & 31, col = first + lane;
+    RowScale r{col < g.n && (threadIdx.x >> 5 & 3) * 32 + lane < g.rows, 1.0f, 0.0f};
     if (r.mine) r.scale = __ldg(g.sb + col);
     if (r.mine && g.bias) r.bias = __ldg(g.bias + col);
-    float touched;  // 8 of them a sector, at most 256 a tile
-    if (token < g.m && 8 * lane < g.bn)
-        asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(touched) : "l"(g.sa + token));
     return r;
+}
+// Whether all products of the warp's scales and the tile's tokens' are only rounded:
+// of all tokens, alike for both warps of a quarter of the lanes, or of those that the
+// warp itself stores (ALL false). (Looked at one by one
+// they cost more than the scaling itself: 2048 x 4096 x 1024 25 us, so 17.)
+template <bool ALL>
+__device__ __forceinline__ bool plain_scales(const TcArgs& g, const RowScale& r, unsigned row0) {
+    const unsigned lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    bool plain = is_plain(r.scale);
+#pragma unroll
+    for (unsigned q = 0; q < (ALL ? 8 : 4); ++q) {
+        const unsigned c = ALL ? lane + 32 * q : (lane & 15) + 16 * (warp >> 2) + 32 * (lane >> 4) + 64 * q;
+        if (c < g.bn && row0 + c < g.m) plain &= is_plain(__ldg(g.sa + row0 + c));
+    }
+    return __all_sync(0xffffffffu, plain);
+}
+
+// One output where scales are not plain.
+__device__ __forceinline__ void store_far(const TcArgs& g, const RowScale& r, int sum, unsigned row, unsigned col) {
+    if (r.mine) {
+        const float p = scaled(sum, __ldg(g.sa + row), r.scale);
+        g.out[static_cast<unsigned long long>(row) * g.n + col] = g.bias ? p + r.bias : p;
+    }
+    __syncwarp();
 }
 
 // A warp's share of a finished tile: 32 weight rows (TMEM lanes, `first` the
 // lowest) and every other 16 tokens, scaled and stored, 128 bytes of one token at
 // a time. The next 16 leave TMEM while the present ones are stored.
-__device__ __forceinline__ void store_tile(const TcArgs& g, const RowScale& r, unsigned tmem, unsigned first,
-                                           unsigned row0) {
+__device__ __forceinline__ void store_tile(const TcArgs& g, const RowScale& r, bool plain, unsigned tmem,
+                                           unsigned first, unsigned row0) {
     const unsigned warp = threadIdx.x >> 5, col = first + (threadIdx.x & 31);
     const unsigned rows = min(g.bn, g.m - row0), step = 16 * (kStoreWarps / 4);
     const unsigned taddr = tmem + ((warp & 3) * 32 << 16);
@@ -281,6 +328,12 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, const RowScale& r, u
     unsigned c = 16 * (warp >> 2);
     int v[16];
     __syncwarp();
+    if (!plain) {
+        // one token at a time: unrolled beside the rest, this kept every tile waiting for instructions
+#pragma unroll 1
+        for (; c < rows; c += c % 16 == 15 ? step - 15 : 1) store_far(g, r, tmem_load1(taddr + c), row0 + c, col);
+        return;
+    }
     if (c < rows) tmem_load16(taddr + c, v);
     for (; c < rows; c += step) {
         float s[16];
@@ -292,7 +345,7 @@ __device__ __forceinline__ void store_tile(const TcArgs& g, const RowScale& r, u
             }
         } else {
 #pragma unroll
-            for (unsigned j = 0; j < 16; ++j) s[j] = c + j < rows ? __ldg(sa + c + j) : 0.0f;
+            for (unsigned j = 0; j < 16; ++j) s[j] = c + j < rows ? __ldg(sa + c + j) : 1.0f;
         }
         __syncwarp();
         tmem_load_wait();
@@ -382,6 +435,7 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
     tc_fence_after();
     const unsigned tmem = tmem_base;
     RowScale r{};
+    bool plain = true;
 
     if (warp == kStoreWarps) {  // fetch
         if (lane == 0) {
@@ -409,10 +463,11 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
             if (ok) mma_commit(acc_full);
         }
     } else {
-        r = row_scale(g, tn * kTileM + (warp & 3) * 32, tm * g.bn);
+        r = row_scale(g, tn * kTileM + (warp & 3) * 32);
+        plain = plain_scales<true>(g, r, tm * g.bn);
         const bool ok = tc_wait<false>(acc_full, 0, dead, g.err);
         tc_fence_after();
-        if (ok && a.split == 1) store_tile(g, r, tmem, tn * kTileM + (warp & 3) * 32, tm * g.bn);
+        if (ok && a.split == 1) store_tile(g, r, plain, tmem, tn * kTileM + (warp & 3) * 32, tm * g.bn);
     }
     if (a.split > 1) {
         const unsigned share = g.bn / a.split, mine0 = rank * share;
@@ -436,7 +491,18 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
         cluster_barrier();
         if (warp < kStoreWarps) {
             const unsigned col = tn * kTileM + l;
-            for (unsigned c = mine0 / 16 * 16 + 16 * (warp >> 2); c < mine0 + share; c += stride) {
+            if (!plain) {
+#pragma unroll 1
+                for (unsigned t = mine0 + (warp >> 2); t < min(mine0 + share, g.m - tm * g.bn); t += kStoreWarps / 4) {
+                    int sum = tmem_load1(taddr + t);
+                    for (unsigned q = 1; q < a.split; ++q) {
+                        const unsigned from = (rank + q) % a.split;
+                        sum += __ldcg(sums + (static_cast<unsigned long long>(from) * g.bn + t) * kTileM + l);
+                    }
+                    store_far(g, r, sum, tm * g.bn + t, col);
+                }
+            }
+            for (unsigned c = mine0 / 16 * 16 + 16 * (warp >> 2); plain && c < mine0 + share; c += stride) {
                 int v[16];
                 tmem_load16(taddr + c, v);
                 int o[kMostSplit - 1][16];  // the others', in flight together
@@ -605,10 +671,11 @@ matmul_q8_pair(const __grid_constant__ CUtensorMap bmap, const __grid_constant__
             const unsigned half = turn & 1;
             unsigned tn, tm;
             tile_at(i, g, tn, tm);
-            const RowScale r = row_scale(g, (2 * tn + rank) * g.rows + (warp & 3) * 32, tm * g.bn);
+            const RowScale r = row_scale(g, (2 * tn + rank) * g.rows + (warp & 3) * 32);
+            const bool plain = plain_scales<false>(g, r, tm * g.bn);
             if (!tc_wait(acc_full + half, (turn >> 1) & 1, dead, g.err)) break;
             tc_fence_after();
-            store_tile(g, r, tmem + half * g.bn, (2 * tn + rank) * g.rows + (warp & 3) * 32, tm * g.bn);
+            store_tile(g, r, plain, tmem + half * g.bn, (2 * tn + rank) * g.rows + (warp & 3) * 32, tm * g.bn);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) arrive_at(in_cta(acc_empty + half, 0));
@@ -631,7 +698,7 @@ matmul_q8_empty(const float* sa, const float* sb, const float* bias, unsigned m,
     const unsigned long long count = static_cast<unsigned long long>(m) * n;
     for (unsigned long long i = blockIdx.x * 256ull + threadIdx.x; i < count; i += gridDim.x * 256ull) {
         const unsigned r = static_cast<unsigned>(i / n), c = static_cast<unsigned>(i - static_cast<unsigned long long>(r) * n);
-        const float v = 0.0f * (sa[r] * sb[c]);
+        const float v = scaled(0, sa[r], sb[c]);
         out[i] = bias ? v + bias[c] : v;
     }
 }
