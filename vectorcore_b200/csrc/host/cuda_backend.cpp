@@ -3,6 +3,7 @@
 
 #include "vc_cuda.h"
 
+#include <cstdint>
 #include <stdexcept>
 #include <string>
 
@@ -51,7 +52,7 @@ std::shared_ptr<CudaStorage> make(std::size_t elements, Device device, std::size
 }  // namespace
 
 CudaStorage::CudaStorage(std::size_t elements, Device device, std::size_t element_bytes)
-    : size_(elements), device_(device) {
+    : size_(elements), element_bytes_(element_bytes), device_(device) {
     check(vc_cuda_alloc((elements ? elements : 1) * element_bytes, &ptr_), "allocation failed");
 }
 
@@ -275,17 +276,47 @@ namespace {
 // 8-bit rows start on 16-byte boundaries.
 std::size_t q8_pitch(std::size_t cols) { return (cols + 15) / 16 * 16; }
 
-const float* optional(const Storage* s) { return s ? ptr(*s) : nullptr; }
+std::size_t times(std::size_t a, std::size_t b) {
+    if (b && a > SIZE_MAX / b) throw std::overflow_error("tensor element count overflows size_t");
+    return a * b;
+}
 
-std::int8_t* q8_ptr(const Storage& s) { return static_cast<std::int8_t*>(as_cuda(s).raw()); }
+// The start of a storage that has to hold `elements` of type T.
+template <typename T = float>
+T* held(const Storage& s, std::size_t elements, const char* what) {
+    const CudaStorage& c = as_cuda(s);
+    if (c.element_bytes() != sizeof(T))
+        throw std::invalid_argument(std::string(what) + " has elements of " + std::to_string(c.element_bytes()) +
+                                    " bytes, not " + std::to_string(sizeof(T)));
+    if (c.size() < elements)
+        throw std::out_of_range(std::string(what) + " has " + std::to_string(c.size()) + " elements, " +
+                                std::to_string(elements) + " are needed");
+    return static_cast<T*>(c.raw());
+}
+template <typename T = float>
+T* held(const Storage* s, std::size_t elements, const char* what) {
+    return s ? held<T>(*s, elements, what) : nullptr;
+}
+
+struct Q8 {
+    const std::int8_t* values;
+    const float* scale;
+};
+Q8 held(const CudaBackend::Q8Matrix& m, const char* what) {
+    if (!m.values || !m.scale) throw std::invalid_argument(std::string(what) + " has no values or no scale");
+    const std::size_t ahead = m.rows ? times(m.rows - 1, m.pitch) : 0, last = m.rows ? m.cols : 0;
+    if (ahead > SIZE_MAX - last) throw std::overflow_error("tensor element count overflows size_t");
+    return Q8{held<std::int8_t>(*m.values, ahead + last, what), held(*m.scale, m.rows, what)};
+}
 
 }  // namespace
 
 CudaBackend::NormResult CudaBackend::rms_norm(const Storage& x, const Storage* residual, const Storage& weight,
                                               std::size_t rows, std::size_t cols, float eps) {
-    NormResult r{make(rows * cols, device_), residual ? make(rows * cols, device_) : nullptr, make(rows, device_)};
-    check(vc_cuda_rms_norm(ptr(x), cols, optional(residual), cols, ptr(weight), rows, cols, eps,
-                           r.h ? ptr(*r.h) : nullptr, ptr(*r.y), ptr(*r.rstd)),
+    const std::size_t n = times(rows, cols);
+    const float *px = held(x, n, "x"), *pr = held(residual, n, "residual"), *pw = held(weight, cols, "weight");
+    NormResult r{make(n, device_), residual ? make(n, device_) : nullptr, make(rows, device_)};
+    check(vc_cuda_rms_norm(px, cols, pr, cols, pw, rows, cols, eps, r.h ? ptr(*r.h) : nullptr, ptr(*r.y), ptr(*r.rstd)),
           "rms_norm failed");
     return r;
 }
@@ -293,46 +324,57 @@ CudaBackend::NormResult CudaBackend::rms_norm(const Storage& x, const Storage* r
 CudaBackend::NormGradients CudaBackend::rms_norm_backward(const Storage& h, const Storage& weight, const Storage& rstd,
                                                           const Storage& gy, const Storage* gh, std::size_t rows,
                                                           std::size_t cols) {
-    NormGradients r{make(rows * cols, device_), make(cols, device_)};
-    check(vc_cuda_rms_norm_backward(ptr(h), ptr(weight), ptr(rstd), ptr(gy), optional(gh), rows, cols, ptr(*r.dh),
-                                    ptr(*r.dw)),
+    const std::size_t n = times(rows, cols);
+    const float *ph = held(h, n, "h"), *pw = held(weight, cols, "weight"), *ps = held(rstd, rows, "rstd");
+    const float *pgy = held(gy, n, "gy"), *pgh = held(gh, n, "gh");
+    NormGradients r{make(n, device_), make(cols, device_)};
+    check(vc_cuda_rms_norm_backward(ph, pw, ps, pgy, pgh, rows, cols, ptr(*r.dh), ptr(*r.dw)),
           "rms_norm_backward failed");
     return r;
 }
 
 CudaBackend::NormQ8Result CudaBackend::rms_norm_q8(const Storage& x, const Storage* residual, const Storage& weight,
                                                    std::size_t rows, std::size_t cols, float eps) {
-    const std::size_t pitch = q8_pitch(cols);
-    NormQ8Result r{{make(rows * pitch, device_, 1), make(rows, device_), rows, cols, pitch},
-                   residual ? make(rows * cols, device_) : nullptr};
-    check(vc_cuda_rms_norm_q8(ptr(x), cols, optional(residual), cols, ptr(weight), rows, cols, eps,
-                              r.h ? ptr(*r.h) : nullptr, q8_ptr(*r.q.values), pitch, ptr(*r.q.scale)),
+    const std::size_t n = times(rows, cols), pitch = q8_pitch(cols);
+    const float *px = held(x, n, "x"), *pr = held(residual, n, "residual"), *pw = held(weight, cols, "weight");
+    NormQ8Result r{{make(times(rows, pitch), device_, 1), make(rows, device_), rows, cols, pitch},
+                   residual ? make(n, device_) : nullptr};
+    check(vc_cuda_rms_norm_q8(px, cols, pr, cols, pw, rows, cols, eps, r.h ? ptr(*r.h) : nullptr,
+                              static_cast<std::int8_t*>(as_cuda(*r.q.values).raw()), pitch, ptr(*r.q.scale)),
           "rms_norm_q8 failed");
     return r;
 }
 
 CudaBackend::Q8Matrix CudaBackend::quantize_q8(const Storage& x, std::size_t rows, std::size_t cols) {
     const std::size_t pitch = q8_pitch(cols);
-    Q8Matrix r{make(rows * pitch, device_, 1), make(rows, device_), rows, cols, pitch};
-    check(vc_cuda_quantize_q8(ptr(x), cols, rows, cols, q8_ptr(*r.values), pitch, ptr(*r.scale)), "quantize_q8 failed");
+    const float* px = held(x, times(rows, cols), "x");
+    Q8Matrix r{make(times(rows, pitch), device_, 1), make(rows, device_), rows, cols, pitch};
+    check(vc_cuda_quantize_q8(px, cols, rows, cols, static_cast<std::int8_t*>(as_cuda(*r.values).raw()), pitch,
+                              ptr(*r.scale)),
+          "quantize_q8 failed");
     return r;
 }
 
 std::shared_ptr<Storage> CudaBackend::matmul_q8(const Q8Matrix& a, const Q8Matrix& b, const Storage* bias) {
     if (a.cols != b.cols) throw std::invalid_argument("matmul_q8: rows of different lengths");
-    auto out = make(a.rows * b.rows, device_);
-    check(vc_cuda_matmul_q8(q8_ptr(*a.values), a.pitch, ptr(*a.scale), q8_ptr(*b.values), b.pitch, ptr(*b.scale),
-                            optional(bias), a.rows, b.rows, a.cols, out->device_data()),
+    const Q8 pa = held(a, "a"), pb = held(b, "b");
+    const float* pbias = held(bias, b.rows, "bias");
+    auto out = make(times(a.rows, b.rows), device_);
+    check(vc_cuda_matmul_q8(pa.values, a.pitch, pa.scale, pb.values, b.pitch, pb.scale, pbias, a.rows, b.rows, a.cols,
+                            out->device_data()),
           "matmul_q8 failed");
     return out;
 }
 
 CudaBackend::SampleResult CudaBackend::sample(const Storage& logits, const Storage& noise,
                                               const SampleSettings& settings, std::size_t rows, std::size_t vocab) {
+    const std::size_t n = times(rows, vocab);
+    const float *px = held(logits, n, "logits"), *pe = held(noise, n, "noise");
+    const float* pt = held(settings.temperature, rows, "temperature");
+    const std::int64_t* pk = held<std::int64_t>(settings.top_k, rows, "top_k");
+    const float *pp = held(settings.top_p, rows, "top_p"), *pm = held(settings.min_p, rows, "min_p");
     SampleResult r{make(rows, device_, sizeof(std::int64_t)), make(rows, device_)};
-    check(vc_cuda_sample(ptr(logits), vocab, ptr(noise), vocab, optional(settings.temperature),
-                         settings.top_k ? static_cast<const std::int64_t*>(as_cuda(*settings.top_k).raw()) : nullptr,
-                         optional(settings.top_p), optional(settings.min_p), rows, vocab,
+    check(vc_cuda_sample(px, vocab, pe, vocab, pt, pk, pp, pm, rows, vocab,
                          static_cast<std::int64_t*>(as_cuda(*r.token).raw()), ptr(*r.logprob)),
           "sample failed");
     return r;

@@ -44,10 +44,11 @@ public:
     [[nodiscard]] std::size_t size() const noexcept override { return size_; }
     [[nodiscard]] float* device_data() const noexcept { return static_cast<float*>(ptr_); }
     [[nodiscard]] void* raw() const noexcept { return ptr_; }
+    [[nodiscard]] std::size_t element_bytes() const noexcept { return element_bytes_; }
 
 private:
     void* ptr_{nullptr};
-    std::size_t size_{0};
+    std::size_t size_{0}, element_bytes_{sizeof(float)};
     Device device_;
 };
 
@@ -134,6 +135,9 @@ public:
                                                                   std::size_t classes);
 
     // ---- language-model operators (no counterpart in the reference) ---------
+    // Rows lie one after another. A storage that is too short is refused with
+    // std::out_of_range, one of elements of another size with
+    // std::invalid_argument.
     // A matrix of int8 values, `pitch` bytes between rows, and a float scale
     // for each row (vc_cuda.h, "q8").
     struct Q8Matrix {
