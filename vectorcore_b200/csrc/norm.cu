@@ -315,7 +315,7 @@ norm_long_kernel(const NormArgs a) {
         for (unsigned long long j = a.cols + threadIdx.x; j < a.pitch; j += blockDim.x) a.q[row * a.pitch + j] = 0;
 }
 
-// Row lengths that a CTA of 1024 threads keeps in registers: nine groups a
+// Row lengths that a CTA of 1024 threads keeps in registers: eight groups a
 // thread forward, four of two tensors backward.
 constexpr unsigned kNormRegCols = 32768, kNormBwdRegCols = 16384;
 bool fits(unsigned cols, unsigned most, bool skewed) { return cols <= (skewed ? most - 3 : most); }
@@ -359,7 +359,7 @@ void launch_norm_skew(const NormArgs& a) {
     const RowShape s = row_shape(a.cols, SKEWED, a.rows);
     if (s.per <= 1) launch_norm_nv<MODE, SKEWED, 1>(a, s);
     else if (s.per <= 4) launch_norm_nv<MODE, SKEWED, 4>(a, s);
-    else launch_norm_nv<MODE, SKEWED, 9>(a, s);
+    else launch_norm_nv<MODE, SKEWED, 8>(a, s);
 }
 
 template <int MODE>
