@@ -196,7 +196,10 @@ class CudaBackend:
     def use_stream(self, handle: int | None) -> None:
         """Enqueue on the stream with this raw handle from now on (another
         library's, e.g. torch.cuda.Stream.cuda_stream; 0 is the default
-        stream). None goes back to the device's own stream."""
+        stream). None goes back to the device's own stream. Call it again
+        whenever the owner works on another stream: what is enqueued on two
+        streams is not ordered, except by this call, which waits for the
+        stream it leaves."""
         # NULL restores the own stream in the C ABI; 1 is cudaStreamLegacy
         _abi.call("vc_cuda_set_stream", ctypes.c_void_p(None if handle is None else handle or 1))
 
