@@ -48,7 +48,7 @@ class CudaStorage:
         nothing is freed when it goes. The owner keeps the memory until the
         work enqueued on it is done."""
         s = _Borrowed.__new__(_Borrowed)
-        s.ptr, s.size, s.dtype, s.version = ptr, elements, dtype, 0
+        s.ptr, s.size, s.dtype, s.version = ptr, elements, np.dtype(dtype), 0
         return s
 
     @property
