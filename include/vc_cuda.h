@@ -448,7 +448,8 @@ vc_status vc_cuda_reduce_sum_noalloc(const float* in, size_t count, float* out);
  * j of row i stands for q[i * pitch + j] * scale[i]. The entry points that
  * write q8 rows zero the bytes past the row's length; matmul_q8 ignores them.
  * A stride argument counts elements between the starts of rows (the row's
- * length for a contiguous tensor). */
+ * length for a contiguous tensor). A tensor may start at any element; one that
+ * starts inside an element is refused with VC_ERR_INVALID. */
 
 /* h = x + residual (residual may be NULL: h = x),
  * rstd = 1 / sqrt(mean(h^2) + eps), y = (h * rstd) * weight, each row of

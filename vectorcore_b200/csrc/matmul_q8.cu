@@ -830,6 +830,7 @@ vc_status vc_cuda_matmul_q8(const int8_t* a, size_t a_pitch, const float* a_scal
         fail(VC_ERR_OVERFLOW, "matmul_q8: matrix too large");
     if (m == 0 || n == 0) return VC_OK;
     if (!a_scale || !b_scale || !out || (k && (!a || !b))) fail(VC_ERR_INVALID, "matmul_q8: null pointer");
+    check_elements("matmul_q8", a_scale, b_scale, bias, out);
     check_q8_in("a", a, a_pitch, k);
     check_q8_in("b", b, b_pitch, k);
     MatmulQ8Args g{};

@@ -996,6 +996,7 @@ vc_status vc_cuda_rms_norm(const float* x, size_t x_stride, const float* residua
     check_eps("rms_norm", eps);
     if (rows == 0) return VC_OK;
     if (!x || !weight || !y) fail(VC_ERR_INVALID, "rms_norm: null pointer");
+    check_elements("rms_norm", x, residual, weight, h, y, rstd);
     check_in_place("rms_norm", h, x, x_stride, rows, cols);
     check_in_place("rms_norm", h, residual, residual_stride, rows, cols);
     NormArgs a{};
@@ -1015,6 +1016,7 @@ vc_status vc_cuda_rms_norm_q8(const float* x, size_t x_stride, const float* resi
     check_eps("rms_norm_q8", eps);
     if (rows == 0) return VC_OK;
     if (!x || !weight) fail(VC_ERR_INVALID, "rms_norm_q8: null pointer");
+    check_elements("rms_norm_q8", x, residual, weight, h, scale);
     check_in_place("rms_norm_q8", h, x, x_stride, rows, cols);
     check_in_place("rms_norm_q8", h, residual, residual_stride, rows, cols);
     check_q8_out("rms_norm_q8", q, scale, cols, q_pitch);
@@ -1033,6 +1035,7 @@ vc_status vc_cuda_quantize_q8(const float* x, size_t x_stride, size_t rows, size
     check_rows_cols("quantize_q8", rows, cols);
     if (rows == 0) return VC_OK;
     if (!x) fail(VC_ERR_INVALID, "quantize_q8: null pointer");
+    check_elements("quantize_q8", x, scale);
     check_q8_out("quantize_q8", q, scale, cols, q_pitch);
     NormArgs a{};
     a.x = x, a.xs = x_stride;
@@ -1047,6 +1050,7 @@ vc_status vc_cuda_rms_norm_backward(const float* h, const float* weight, const f
     VC_API_BEGIN
     ensure_init();
     check_rows_cols("rms_norm_backward", rows, cols);
+    check_elements("rms_norm_backward", h, weight, rstd, gy, gh, dh, dw);
     if (rows == 0) {  // the sum over no rows
         if (dw) VC_CUDA(cudaMemsetAsync(dw, 0, cols * sizeof(float), stream()));
         return VC_OK;

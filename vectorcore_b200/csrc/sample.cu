@@ -986,6 +986,7 @@ vc_status vc_cuda_sample(const float* logits, size_t logits_stride, const float*
     if (rows > 0x7fffffffull) fail(VC_ERR_OVERFLOW, "sample: too many rows");
     if (rows == 0) return VC_OK;
     if (!logits || !noise || !token || !logprob) fail(VC_ERR_INVALID, "sample: null pointer");
+    check_elements("sample", logits, noise, temperature, top_k, top_p, min_p, token, logprob);
     SampleArgs a{};
     a.logits = logits, a.ls = logits_stride, a.noise = noise, a.ns = noise_stride;
     a.temperature = temperature, a.top_k = reinterpret_cast<const long long*>(top_k);

@@ -116,6 +116,14 @@ private:
     bool active_{false}, joined_{false};
 };
 
+// Refuses tensors that do not start on a boundary of their elements, which borrowed
+// memory may: a kernel's access to one would fault.
+template <typename... T>
+inline void check_elements(const char* what, const T*... p) {
+    if (((reinterpret_cast<std::uintptr_t>(p) % sizeof(T)) | ... | 0))
+        fail(VC_ERR_INVALID, std::string(what) + ": a tensor starts inside an element");
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<std::uintptr_t>(p) & 15u) == 0; }
 
 // Streaming layout of the flat elementwise kernels (same-shape, scalar and
