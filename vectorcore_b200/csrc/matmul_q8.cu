@@ -46,7 +46,7 @@ __device__ __forceinline__ bool is_plain(float s) { return s == 0.0f || (fabsf(s
 // m16n8k32 products. A product's four groups of k may be any four as long as both
 // sides agree, so a thread's 16 consecutive bytes serve as they are; no byte is
 // moved between threads. The warps' sums meet in shared memory. 1 x 32000 x 4096
-// takes 24 us, 5.5 TB/s (the tensor-core tiles below 30); 1 x 4096 x 4096 5.9.
+// takes 23 us, 5.7 TB/s (the tensor-core tiles below 30); 1 x 4096 x 4096 5.9.
 constexpr unsigned kRowsWarps = 8;
 constexpr unsigned kPiece = 128;  // bytes of k a warp takes at a time
 
@@ -548,8 +548,8 @@ matmul_q8_split(const __grid_constant__ CUtensorMap bmap, const __grid_constant_
 // tile. The previous tile leaves the other half of TMEM meanwhile. A stage holds
 // 256 bytes of k, eight products: with 128 the one thread's wait, issue and commit
 // took longer than the four products they bring (8192^3: 385 us with one CTA a
-// tile and 128 bytes, 313 this way: 3.5 Pop/s, twice the rate of a 16-bit library
-// product here; in a long run the 1000 W limit leaves 2.8).
+// tile and 128 bytes, 313 this way on the same card; 345 alone on another, 3.2 Pop/s,
+// and 2.6 in a long run under the 1000 W limit).
 constexpr unsigned kPairSlices = 2;
 
 __device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, unsigned bar, int x, int y) {

@@ -166,8 +166,9 @@ __host__ __device__ __forceinline__ unsigned q8_bytes(unsigned cols) { return (c
 
 // One row a CTA (or a row a warp, blockDim.y of them, for short rows): the row
 // is read once and stays in registers, NV groups a thread; HBM bounds it. 8192 x
-// 8192: 162 us for the norm (6.6 TB/s), 133 in 8 bits (6.55), 61 for the 8 bits
-// alone; rows off the 16-byte grid run at 5.2 TB/s (8000 x 5003: 123 us).
+// 8192: 158 us for the norm (6.8 TB/s), 129 in 8 bits (6.8), 57 for the 8 bits
+// alone; rows off the 16-byte grid run at 5.4 TB/s (8000 x 5003: 118 us), their 8 bits
+// at 4.3, bound by instructions.
 template <int MODE, bool SKEWED, int NV>
 __global__ void __launch_bounds__(1024)
 norm_kernel(const NormArgs a) {
@@ -276,8 +277,9 @@ norm_kernel(const NormArgs a) {
     }
 }
 
-// Rows too long for the registers of one CTA: the same in two passes, the
-// second reading h back (or x and the residual again where h is not wanted).
+// Rows too long for the registers of one CTA, or tensors of unlike alignment: the
+// same in two passes by single floats, the second reading h back (or x and the
+// residual again where h is not wanted). 8192 x 8192 of unlike ones: 269 us, 4.0 TB/s.
 template <int MODE>
 __global__ void __launch_bounds__(1024)
 norm_long_kernel(const NormArgs a) {
@@ -390,12 +392,12 @@ struct NormBwdArgs {
     float* dh;
 };
 
-// dh and dw in one launch, for what the ring below does not take: few rows, odd
-// lengths. The first CTAs write dh: groups of T threads, 1024 / T of them a CTA,
-// have a row each, h and t = gy * w in registers. The others add up dw: 32
-// columns a CTA, a slice of at most kDwRows of its rows a warp in float, the
-// slices in double and in order. Rows beyond 32 slices go to further CTAs whose
-// sums norm_dw_finish adds.
+// dh and dw in one launch, for what the ring below does not take: few rows, lengths
+// beyond its own, one of the two alone (8192 x 8192: dh 187 us, 5.7 TB/s, dw 92, 5.9).
+// The first CTAs write dh: groups of T threads, 1024 / T of them a CTA, have a row
+// each, h and t = gy * w in registers. The others add up dw: 32 columns a CTA, a slice
+// of at most kDwRows of its rows a warp in float, the slices in double and in order.
+// Rows beyond 32 slices go to further CTAs whose sums norm_dw_finish adds.
 constexpr unsigned kDwRows = 64;          // float additions in a row of a sum
 constexpr unsigned kDwSpan = 32 * kDwRows;  // rows a CTA adds up
 
@@ -490,7 +492,8 @@ norm_bwd_both(const BothArgs b) {
     else dw_of_columns(b, part);
 }
 
-// dh for rows too long for registers, or tensors of unlike alignment.
+// dh for rows too long for registers, or tensors of unlike alignment (8192 x 8192 with
+// dw in a launch before it: 409 us).
 __global__ void __launch_bounds__(1024)
 norm_bwd_dh_long(const NormBwdArgs a) {
     __shared__ double scratch[32];
@@ -555,7 +558,7 @@ void launch_dw_finish(const float* partial, unsigned long long count, unsigned c
 // that come with a copy (with every thread looking for them 30000 x 2047 took 347
 // us, now 253; with columns by single floats 458, with dh and dw by themselves 327).
 //
-// HBM bounds the even lengths (8192 x 8192: 5.67 TB/s, 30000 x 2048 in 161 us: 6.1
+// HBM bounds the even lengths (8192 x 8192: 5.84 TB/s, 30000 x 2048 in 157 us: 6.3
 // TB/s), instructions the odd ones, those at the rows' ends above all.
 constexpr unsigned kRingThreads = 512;
 constexpr unsigned kRingWarps = kRingThreads / 32;
@@ -585,8 +588,8 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, unsigned b
 // Rows of up to twice kRingCols floats: a pair of CTAs has a row, each one half of
 // its columns, and every warp tells both CTAs its part of the dot product. Four
 // places for them go round: before a warp writes to one again, both CTAs have
-// used it. 4000 x 16384 takes 202 us, 5.2 TB/s (dh and dw by themselves 286); 11008
-// columns, 2.7 groups a thread, 4.2 TB/s.
+// used it. 4000 x 16384 takes 196 us, 5.3 TB/s (dh and dw by themselves 286); 11008
+// columns, 2.7 groups a thread, 4.3 TB/s.
 struct PairSlots {
     double dot[4][2 * kRingWarps];
     unsigned long long told[4];
