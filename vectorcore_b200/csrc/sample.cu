@@ -779,6 +779,8 @@ sample_kernel(const SampleArgs a) {
         for (unsigned r = 0; r < C; ++r) all += parts[r];
         return all;
     };
+    // Where a row has a class in play its maximum has been found in a pass: its distance
+    // is 0 and its weight 1, which reaches any min-p that is still on.
     const auto first_class = [&] {
         unsigned i = at_once ? key_index(top) : s.firsts[0];
         for (unsigned r = 1; r < C && !at_once; ++r) i = min(i, s.firsts[r]);
